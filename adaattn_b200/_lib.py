@@ -86,6 +86,20 @@ _SIGNATURES = {
     "ada_linear": (c_int32, [_T, _T, _T, _T, c_int32, _T, c_void_p]),
     "ada_layer_norm": (c_int32, [_T, _T, _T, c_float, _T, c_void_p]),
     "ada_record_statistics": (c_int32, [c_void_p, _T, _T, _T, c_void_p]),
+    "ada_paged_attn_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    "ada_paged_attn": (c_int32, [_T, _T, _T, _T, _T, _T, _T, _T, _T, c_float, _T, c_void_p, c_void_p,
+                                 c_size_t, c_void_p]),
+    "ada_paged_append": (c_int32, [_T, _T, _T, _T, _T, _T, _T, _T, _T, _T, c_void_p]),
+    "ada_pages_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "ada_pages_free": (c_int32, [_T, _T, _T, c_int64, _T, c_void_p]),
+    "ada_pages_fork": (c_int32, [_T, _T, _T, c_int64, _T, _T, c_void_p]),
+    "ada_pages_reserve": (c_int32, [_T, _T, _T, _T, c_int64, _T, _T, _T, c_void_p, c_size_t, c_void_p]),
+    "ada_pages_copy": (c_int32, [_T, _T, _T, _T, c_int64, _T, _T, _T, c_void_p, c_size_t, c_void_p]),
+    "ada_pages_compact": (c_int32, [_T, _T, _T, _T, c_int64, _T, c_void_p, c_size_t, c_void_p]),
+    "ada_token_logprobs": (c_int32, [_T, _T, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_void_p]),
+    "ada_token_logprobs_bwd": (c_int32, [_T, _T, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                         c_void_p, _T, c_void_p]),
     "ada_rsvd_workspace_bytes": (c_size_t, [_T, _T, c_int32]),
     "ada_rsvd": (c_int32, [_T, _T, c_int32, c_int32, _T, _T, _T, c_void_p, c_size_t, c_void_p]),
 }

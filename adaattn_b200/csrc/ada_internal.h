@@ -304,4 +304,120 @@ struct BwdLaunch {
 };
 int launch_attn_bwd(const BwdLaunch& L, cudaStream_t stream);
 
+// --- paged key-value cache --------------------------------------------------------
+struct PagedAttnLaunch {
+    const void* q;       // [B, H, D]
+    const void* k;       // [P, Hkv, page, D]
+    const void* v;
+    int q_dtype, kv_dtype;
+    int64_t qs[2], ks[3], vs[3];  // element strides (the innermost is 1)
+    int vec;             // pages' rows aligned to 4 elements, D a multiple of 4
+    const int32_t* table;  // [S, W] rows at table_ld
+    const int32_t* lens;   // [S]
+    const int32_t* seqs;   // [B] table rows, or null: row b
+    int64_t S, W, P, table_ld;
+    int page;
+    MaskView mask;       // [B, mask_len] strides s[0], s[1]; keys from mask_len on are open
+    int64_t mask_len;
+    const float* k_scale;  // [Hkv] or null
+    const float* v_scale;
+    float scale;
+    int B, H, D;
+    int G;               // query heads per key/value head
+    int GB, HB;          // query heads per block and blocks per key/value head
+    int64_t U;           // units per sequence: key/value heads x HB
+    void* out;           // [B, H, D] in q's dtype
+    int64_t os[2];
+    float* lse;          // [B, H] or null
+    int64_t n_cta;
+    int* pref;           // workspace: [B + 1] tiles before each sequence
+    float* part_ml;      // workspace: [n_cta][2][GB][2]
+    float* part_acc;     // workspace: [n_cta][2][GB][D]
+    unsigned int* status;
+    uint64_t timeout_ns;
+};
+int launch_paged_attn(const PagedAttnLaunch& L, cudaStream_t stream);
+
+struct AppendLaunch {
+    const void* k;       // [B, Hkv, N, D]
+    const void* v;
+    void* k_pages;       // [P, Hkv, page, D]
+    void* v_pages;
+    int src_dtype, dst_dtype;
+    int64_t ks[3], vs[3], kps[3], vps[3];
+    const int32_t* table;
+    const int32_t* lens;        // lengths with the new tokens
+    const int32_t* new_tokens;  // [B] or null: N each
+    const int32_t* seqs;
+    int64_t S, W, P, table_ld, B, N, Hkv;
+    int page, D;
+    int vec;             // rows of both sides aligned for eight elements, D a multiple of 8
+    int chunks;          // blocks per sequence
+    const float* k_scale;
+    const float* v_scale;
+    unsigned int* status;
+};
+int launch_paged_append(const AppendLaunch& L, cudaStream_t stream);
+
+struct PagesLaunch {
+    int32_t* table;      // [S, W] rows at table_ld
+    int32_t* lens;       // [S]
+    int32_t* refs;       // [P]
+    int64_t S, W, P, table_ld, page;
+    const int32_t* src;  // [n]
+    const int32_t* dst;  // [n] (free: the sequences)
+    const int32_t* extra;  // [n] tokens to reserve
+    int64_t n;
+    int32_t* granted;    // [n]; compact: [1] live pages
+    // page data: [planes][P][page_bytes]
+    void* data;
+    int64_t planes, plane_bytes, page_stride, page_bytes;
+    int vec;             // bytes per move
+    int move_blocks;
+    // workspace
+    int32_t* n_pairs;
+    int32_t* pairs;      // [P][2] from, to
+    int32_t* free_list;  // [P]
+    int32_t* to;         // [P]
+    int32_t* sharers;    // [P]
+    int32_t* last;       // [P]
+    int32_t* copied;     // [P]
+    int32_t* claim;      // [S]
+    int32_t* need;       // [n]
+    int32_t* first;      // [n]
+    unsigned int* status;
+};
+int launch_pages_share(const PagesLaunch& L, bool fork, cudaStream_t stream);
+int launch_pages_alloc(const PagesLaunch& L, bool copy, cudaStream_t stream);
+int launch_pages_compact(const PagesLaunch& L, cudaStream_t stream);
+
+// --- log probabilities of given tokens ----------------------------------------------
+struct LogprobLaunch {
+    const void* logits;  // [A, R, V], unit innermost stride: row r at (r / R) s0 + (r % R) s1
+    int dtype;
+    int64_t R, s0, s1, rows;
+    int V;
+    const void* tokens;  // [rows]
+    int tok64;           // int64 tokens (else int32)
+    int64_t ignore;
+    int top;
+    float* logprobs;     // [rows]
+    float* entropy;      // [rows]
+    float* lse;          // [rows]
+    float* stats;        // [rows][2]: row maximum, log of the sum of exp(z - maximum)
+    float* top_logprobs; // [rows][top]
+    int64_t* top_tokens;
+    int cluster;         // CTAs per row
+    // backward
+    const float* g_logprobs;  // [rows] or null, and so on
+    const float* g_entropy;
+    const float* g_lse;
+    void* grad;          // [A, R, V] in the logits' dtype: strides gs0, gs1
+    int64_t gs0, gs1;
+    int segments;        // blocks per row
+    unsigned int* status;
+};
+int launch_token_logprobs(const LogprobLaunch& L, cudaStream_t stream);
+int launch_token_logprobs_bwd(const LogprobLaunch& L, cudaStream_t stream);
+
 }  // namespace ada

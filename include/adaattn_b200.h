@@ -280,6 +280,103 @@ int         ada_record_statistics(const float* summary, AdaTensor* call_count,
                                   AdaTensor* low_rank_calls, AdaTensor* precision_distribution,
                                   void* stream);
 
+/* ---- serving: the paged key-value cache and token scores -------------------
+ * These have no counterpart in the reference, whose attention takes whole
+ * sequences. The cache is a pool of pages: k_pages and v_pages
+ * [P, Hkv, page, D] (any strides, the innermost 1; fp32, fp16, bf16 or E4M3),
+ * page_table int32 [S, W] (the page ids of sequence s in order), seq_lens
+ * int32 [S] and ref_counts int32 [P] (how many sequences hold a page; 0: free)
+ * are all device memory that the caller owns. Sequence s holds the first
+ * ceil(seq_lens[s] / page) entries of its row. Nothing here synchronises or
+ * allocates; each call may be captured into a CUDA graph. What a kernel finds
+ * wrong in device data (a page id, a length, a sequence or a token out of
+ * range) it leaves out, and records ADA_ERR_INVALID in the status word that
+ * ada_poll_device_status reads. Views with at most 2^31 - 1 pages, tokens per
+ * sequence and rows; head dims 1..128; pages of 1..65536 tokens. */
+
+/* out[b, h] = softmax(scale * q[b, h] . K) V over the seq_lens keys of table
+ * row seqs[b] (row b when seqs is NULL or its data is): q, out [B, H, D] in
+ * one type, which is the pages' unless they are E4M3; H a multiple of Hkv
+ * (query heads h of a group of H / Hkv share a key/value head); B <= 4096.
+ * key_mask [B, L] (or [1, L]) bool (nonzero keeps) or floating point (added;
+ * -inf hides), for keys j < L, later keys are open. Hidden keys are not read.
+ * k_scale, v_scale float32 [Hkv]: an E4M3 page holds value / scale (NULL: 1).
+ * lse float32 [B, H] or NULL: log sum exp of the scores (-inf and a zero
+ * output row where no key is visible). */
+size_t      ada_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim);
+int         ada_paged_attn(const AdaTensor* q, const AdaTensor* k_pages, const AdaTensor* v_pages,
+                           const AdaTensor* page_table, const AdaTensor* seq_lens, const AdaTensor* seqs,
+                           const AdaTensor* key_mask, const AdaTensor* k_scale, const AdaTensor* v_scale,
+                           float scale, AdaTensor* out, float* lse,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Writes token t < new_tokens[b] (N when NULL) of k, v [B, Hkv, N, D] at
+ * position seq_lens - new_tokens[b] + t of table row seqs[b] (row b when
+ * NULL): seq_lens are the lengths with the new tokens, as ada_pages_reserve
+ * leaves them. The written pages must be held by their sequence alone. k and v
+ * have the pages' type, or the pages are E4M3: value / scale rounded once,
+ * saturating at 448. A sequence named twice is written by its first row. */
+int         ada_paged_append(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages, AdaTensor* v_pages,
+                             const AdaTensor* page_table, const AdaTensor* seq_lens,
+                             const AdaTensor* new_tokens, const AdaTensor* seqs,
+                             const AdaTensor* k_scale, const AdaTensor* v_scale, void* stream);
+
+/* Page operations. `pages` is the page data [planes, P, elements of a page]
+ * (a plane per layer and tensor). Free pages are handed out lowest id first.
+ *   free     the sequences give their pages up (length 0, entries -1).
+ *   fork     dst[i] gives its pages up and holds src[i]'s (no data moves).
+ *   reserve  sequence seqs[i] grows by new_tokens[i] tokens: fresh pages for
+ *            what does not fit those it holds, and a copy of its last page
+ *            where that is part full and shared (the last of a call's
+ *            sequences that share it keeps it, when they are all its holders).
+ *            granted[i] = new_tokens[i], or 0 when the free pages do not
+ *            suffice for the needs of the sequences up to and including i
+ *            (one that needs none is always served) and it stays as it was.
+ *   copy     dst[i] gives its pages up and gets its own copy of src[i]'s;
+ *            granted[i] is its length, 0 (and an empty dst[i]) when the free
+ *            pages do not suffice.
+ *   compact  moves the live pages into the ids 0 .. live - 1 (those above move
+ *            into the holes below, both ascending) and rewrites every row of
+ *            page_table; live is an int32 [1].
+ * A sequence named twice counts once (the first time); a dst that is a src of
+ * the same call is left out. The workspace is ada_pages_workspace_bytes(P, S,
+ * n) for n sequences (0 for compact); calls that overlap need one each. */
+size_t      ada_pages_workspace_bytes(int64_t num_pages, int64_t num_sequences, int64_t n);
+int         ada_pages_free(AdaTensor* page_table, AdaTensor* seq_lens, AdaTensor* ref_counts,
+                           int64_t page_size, const AdaTensor* seqs, void* stream);
+int         ada_pages_fork(AdaTensor* page_table, AdaTensor* seq_lens, AdaTensor* ref_counts,
+                           int64_t page_size, const AdaTensor* src, const AdaTensor* dst, void* stream);
+int         ada_pages_reserve(const AdaTensor* pages, AdaTensor* page_table, AdaTensor* seq_lens,
+                              AdaTensor* ref_counts, int64_t page_size, const AdaTensor* seqs,
+                              const AdaTensor* new_tokens, AdaTensor* granted,
+                              void* workspace, size_t workspace_bytes, void* stream);
+int         ada_pages_copy(AdaTensor* pages, AdaTensor* page_table, AdaTensor* seq_lens,
+                           AdaTensor* ref_counts, int64_t page_size, const AdaTensor* src,
+                           const AdaTensor* dst, AdaTensor* granted,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int         ada_pages_compact(AdaTensor* pages, AdaTensor* page_table, AdaTensor* seq_lens,
+                              AdaTensor* ref_counts, int64_t page_size, AdaTensor* live,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* Scores of given tokens: for each row of logits [A, R, V] (fp32, fp16 or
+ * bf16; any row strides) and its entry of tokens [A * R] (int64 or int32):
+ *   logprobs      log softmax(row)[token]; 0 where token == ignore_index, NaN
+ *                 where it is out of range
+ *   entropy, lse  of softmax(row): -sum p log p; log sum exp
+ *   top_logprobs, top_tokens [rows, top_k] (NULL when top_k = 0; top_k <= 64):
+ *                 the largest in order, equal logits by lowest token, NaN first
+ *   stats         [rows, 2] row maximum and log sum exp(z - maximum), for the gradient
+ * all float32 (top_tokens int64). A logit of -inf has probability 0; a row of
+ * -inf alone, or one with +inf or NaN, gives NaN (lse: -inf for the former). */
+int         ada_token_logprobs(const AdaTensor* logits, const AdaTensor* tokens, int64_t ignore_index,
+                               int32_t top_k, float* logprobs, float* entropy, float* lse, float* stats,
+                               float* top_logprobs, int64_t* top_tokens, void* stream);
+/* Gradient of logprobs, entropy and lse (upstream float32 [rows], NULL: none)
+ * with respect to the logits: grad [A, R, V] in the logits' type. */
+int         ada_token_logprobs_bwd(const AdaTensor* logits, const AdaTensor* tokens, int64_t ignore_index,
+                                   const float* stats, const float* entropy, const float* g_logprobs,
+                                   const float* g_entropy, const float* g_lse, AdaTensor* grad, void* stream);
+
 /* Test hook for failure detection: launches one block that waits on a device
  * barrier nothing ever signals, bounded by `timeout_ns`; the wait gives up,
  * records ADA_ERR_TIMEOUT in the status word and the kernel returns normally. */

@@ -1,0 +1,367 @@
+"""Log probabilities of given tokens (ada_token_logprobs) and their gradient
+against 64-bit evaluations.
+
+Tolerances. Forward, with x = z - max of size up to X and V terms: the sums
+hold each term with the exponential's 2^-21 (its argument x log2 e is rounded
+to 2^-24 X) and at most V / 256 / parts + 40 dependent additions; so s is off
+by r = 2^-21 + X 2^-23 + (V / 256 + 40) 2^-24 relative, a log by as much
+absolutely plus 2^-23 of its value, and the entropy by r times the mean of
+|x| as well. The values then carry fp32 roundings of numbers up to |z|.
+Gradient: fp32 terms off by the same r of their size, rounded once to the
+logits' type (half a step).
+"""
+
+import math
+
+import pytest
+import torch
+
+import adaattn_b200 as ada
+from adaattn_b200 import _lib
+from adaattn_b200.scoring import token_logprobs_backward
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _make(rows, vocab, dtype, seed=0, spread=3.0):
+    g = torch.Generator().manual_seed(seed + rows + vocab)
+    z = torch.randn(rows, vocab, generator=g) * spread * (0.2 + torch.rand(rows, 1, generator=g))
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    if rows > 2:
+        t[1] = -100
+    return z.to(dtype), t
+
+
+def _exact(z, t, ignore=-100):
+    z = z.double()
+    lse = torch.logsumexp(z, -1)
+    logp = z - lse[:, None]
+    p = logp.exp()
+    ent = -torch.where(p > 0, p * logp, torch.zeros_like(p)).sum(-1)
+    lp = logp.gather(1, t.clamp(0, z.shape[1] - 1)[:, None])[:, 0]
+    return torch.where(t == ignore, torch.zeros_like(lp), lp), ent, lse, logp
+
+
+def _r(z):
+    zf = z.double()
+    zf = zf[torch.isfinite(zf)]
+    x = (zf.max() - zf.min()).item() if zf.numel() else 0.0
+    return 2.0 ** -21 + min(x, 120.0) * 2.0 ** -23 + (z.shape[-1] / 256 + 40) * 2.0 ** -24, x
+
+
+def _top(z, k):
+    o = torch.sort(z.double(), dim=-1, descending=True, stable=True).indices
+    return o[..., :k]
+
+
+def _off(got, want):
+    """Largest difference; equal infinities differ by nothing."""
+    got = got.cpu().double()
+    return torch.where(got == want, torch.zeros_like(want), (got - want).abs()).max().item()
+
+
+def _check(z, t, dev, top=0, zd=None):
+    zd = z.to(dev) if zd is None else zd
+    got = ada.token_logprobs(zd, t.to(dev), top_k=top)
+    torch.cuda.synchronize()
+    _lib.poll_device_status(dev)
+    lp, ent, lse, logp = _exact(z, t)
+    r, x = _r(z)
+    big = z.double()[torch.isfinite(z.double())].abs().max().item() + math.log(z.shape[1])
+    bar = 2 * r + 2.0 ** -22 * big
+    assert _off(got.logprobs, lp) <= bar
+    assert _off(got.lse, lse) <= bar
+    assert _off(got.entropy, ent) <= bar + 2 * r * (ent.max().item() + 1)
+    if top:
+        ids = _top(z, top)
+        assert torch.equal(got.top_tokens.cpu(), ids)
+        assert _off(got.top_logprobs, logp.gather(1, ids)) <= bar
+    else:
+        assert got.top_tokens is None and got.top_logprobs is None
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 7, 3), (3, 64, 64), (5, 1000, 20), (2, 4096, 5), (4, 4097, 0),
+                                            (1, 50257, 20), (37, 50257, 5), (300, 5003, 1), (2, 131072, 64),
+                                            (3, 200003, 7), (160, 8192, 32), (700, 300, 64)])
+def test_matches_formula(rows, vocab, top, dtype, cuda_device):
+    z, t = _make(rows, vocab, dtype)
+    _check(z, t, cuda_device, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pad,offset", [(47, 0), (1, 0), (0, 1), (3, 5), (8, 7)])
+def test_row_strides_and_alignment(pad, offset, dtype, cuda_device):
+    z, t = _make(9, 2043, dtype)
+    buf = torch.full((9 * (2043 + pad) + offset + 8,), math.nan, dtype=dtype, device=cuda_device)
+    zd = buf[offset:offset + 9 * (2043 + pad)].view(9, 2043 + pad)[:, :2043]
+    zd.copy_(z)
+    _check(z, t, cuda_device, 10, zd)
+
+
+def test_leading_dimensions(cuda_device):
+    """The next-token slice of a decoder's padded logits, one row, four
+    dimensions, a transposed layout. Layouts of other alignment add a row's
+    terms in another order, so each result is within the forward's bar of the
+    64-bit value and two of them within twice that of one another."""
+    dev = cuda_device
+    z, t = _make(4 * 6, 1003, torch.bfloat16)
+    r, _ = _r(z)
+    bar = 2 * (2 * r + 2.0 ** -22 * (z.double().abs().max().item() + math.log(1003))) + 4 * r * math.log(1003)
+    near = lambda a, b: a.shape == b.shape and (a - b).abs().max().item() <= bar
+    store = torch.full((4, 7, 1024), math.nan, dtype=torch.bfloat16, device=dev)
+    view = store[:, :-1, :1003]
+    view.copy_(z.view(4, 6, 1003))
+    got = ada.token_logprobs(view, t.view(4, 6).to(dev), top_k=3)
+    flat = ada.token_logprobs(z.to(dev), t.to(dev), top_k=3)
+    assert near(got.logprobs.reshape(-1), flat.logprobs) and got.logprobs.shape == (4, 6)
+    assert torch.equal(got.top_tokens.reshape(-1, 3), flat.top_tokens) and got.top_tokens.shape == (4, 6, 3)
+    got = ada.token_logprobs(z[0].to(dev), t[0].to(dev), top_k=3)
+    assert got.logprobs.shape == () and torch.equal(got.top_tokens, flat.top_tokens[0])
+    got = ada.token_logprobs(view.unflatten(1, (2, 3)), t.view(4, 2, 3).to(dev))
+    assert near(got.lse.reshape(-1), flat.lse) and got.lse.shape == (4, 2, 3)
+    got = ada.token_logprobs(z.to(dev).t().contiguous().t(), t.to(torch.int32).to(dev))
+    assert near(got.entropy, flat.entropy)
+    empty = ada.token_logprobs(z[:0].to(dev), t[:0].to(dev), top_k=3)
+    assert empty.logprobs.shape == (0,) and empty.top_tokens.shape == (0, 3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ties_take_the_lowest_tokens(dtype, cuda_device):
+    dev = cuda_device
+    for vocab in (100, 5000, 50257):
+        z = torch.zeros(4, vocab, dtype=dtype)
+        z[1, vocab // 2:] = 1.0              # a tie of half the row
+        z[2] = torch.arange(vocab) % 7       # many ties at every value
+        z[3] = -0.0
+        z[3, ::2] = 0.0                      # both zeros are one value
+        t = torch.zeros(4, dtype=torch.int64)
+        _check(z, t, dev, 64)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [4099, 50257])
+def test_orders_that_fill_the_candidate_list(dtype, vocab, cuda_device):
+    up = torch.linspace(-20, 20, vocab)
+    z = torch.stack([up, up.flip(0), up.abs(), -up.abs()]).to(dtype)
+    _check(z, torch.full((4,), vocab - 1), cuda_device, 64)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masked_vocabularies(dtype, cuda_device):
+    """-inf over most of a row, all of it but one or fewer entries than alternatives."""
+    dev = cuda_device
+    vocab = 9000
+    z, t = _make(6, vocab, dtype)
+    z[0, 5:] = -math.inf
+    z[1, :-1] = -math.inf
+    z[2, :4096] = -math.inf
+    z[3, ::2] = -math.inf
+    t[:] = torch.tensor([3, vocab - 1, 8000, 1, 0, 4])
+    got = _check(z, t, dev, 64)
+    assert abs(got.entropy[1].item()) <= 1e-6 and abs(got.logprobs[1].item()) <= 1e-6
+    t[0] = 10  # a hidden token
+    assert ada.token_logprobs(z.to(dev), t.to(dev)).logprobs[0].item() == -math.inf
+    lowest = torch.full((1, vocab), torch.finfo(dtype).min, dtype=dtype)
+    got = ada.token_logprobs(lowest.to(dev), t[:1].to(dev), top_k=2)
+    assert abs(got.entropy.item() - math.log(vocab)) <= 1e-5
+    assert abs(got.logprobs.item() + math.log(vocab)) <= 1e-5 and got.top_tokens.tolist() == [[0, 1]]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_without_a_distribution(dtype, cuda_device):
+    dev = cuda_device
+    z, t = _make(5, 6000, dtype)
+    z[0] = -math.inf
+    z[1, 77] = math.nan
+    z[2, 4500] = math.inf
+    z[3, :4200] = math.nan
+    x = z.to(dev).requires_grad_()
+    t = t.clamp_min(0)
+    got = ada.token_logprobs(x, t.to(dev), top_k=3)
+    assert torch.isnan(got.logprobs[:4]).all() and torch.isnan(got.entropy[:4]).all()
+    assert got.lse[0].item() == -math.inf and torch.isfinite(got.logprobs[4])
+    assert got.top_tokens[1, 0].item() == 77 and got.top_tokens[2, 0].item() == 4500
+    assert got.top_tokens[3].tolist() == [0, 1, 2] and got.top_tokens[0].tolist() == [0, 1, 2]
+    grad, = torch.autograd.grad(got.logprobs.sum(), x)
+    assert torch.isnan(grad[:4].float()).all(-1).all() and torch.isfinite(grad[4].float()).all()
+
+
+def test_tokens_outside_the_vocabulary(cuda_device):
+    dev = cuda_device
+    z, t = _make(4, 500, torch.float32)
+    t = torch.tensor([-1, 500, 3, -100])
+    x = z.to(dev).requires_grad_()
+    got = ada.token_logprobs(x, t.to(dev))
+    with pytest.raises(ada.KernelError):
+        _lib.poll_device_status(dev)
+    assert torch.isnan(got.logprobs[:2]).all() and torch.isfinite(got.logprobs[2:]).all()
+    assert got.logprobs[3].item() == 0
+    grad, = torch.autograd.grad(got.logprobs.sum(), x)
+    assert torch.isnan(grad[:2]).all() and torch.isfinite(grad[2:]).all() and (grad[3] == 0).all()
+    assert torch.equal(ada.token_logprobs(z.to(dev), t.to(dev).clamp_min(0).clamp_max(499), ignore_index=3).logprobs[2:3],
+                       torch.zeros(1, device=dev))
+
+
+def _grad64(z, t, g_lp, g_ent, g_lse):
+    z = z.double()
+    _, ent, lse, logp = _exact(z, t)
+    p = logp.exp()
+    hit = torch.zeros_like(z)
+    hit[torch.arange(len(t)), t.clamp_min(0)] = 1
+    g = g_lp.double() * (t != -100)
+    plogp = torch.where(p > 0, logp, torch.zeros_like(p))
+    return (g[:, None] * (hit - p) - g_ent.double()[:, None] * p * (plogp + ent[:, None])
+            + g_lse.double()[:, None] * p)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,pad", [(1, 1, 0), (3, 17, 0), (6, 1000, 0), (5, 4099, 0), (4, 50257, 47),
+                                            (3, 50257, 0), (400, 515, 13)])
+def test_gradient_matches_formula(rows, vocab, pad, dtype, cuda_device):
+    dev = cuda_device
+    z, t = _make(rows, vocab, dtype)
+    if rows > 2:
+        z[0, vocab // 2:] = -math.inf
+        t[0] = 0
+    g = torch.Generator().manual_seed(3)
+    ups = [torch.randn(rows, generator=g) for _ in range(3)]
+    store = torch.zeros(rows, vocab + pad, dtype=dtype, device=dev)
+    x = store[:, :vocab]
+    x.copy_(z)
+    x = x.requires_grad_()
+    got = ada.token_logprobs(x, t.to(dev))
+    grad, = torch.autograd.grad((got.logprobs, got.entropy, got.lse), x, [u.to(dev) for u in ups])
+    assert grad.shape == x.shape and grad.dtype == dtype
+    want = _grad64(z, t, *ups)
+    r, _ = _r(z)
+    _, ent, _, logp = _exact(z, t)
+    p = logp.exp()
+    size = p * (sum(u.abs().double() for u in ups)[:, None]
+                * (1 + torch.where(p > 0, logp.abs(), torch.zeros_like(p)) + ent.abs()[:, None]))
+    hit = torch.zeros_like(want)
+    hit[torch.arange(rows), t.clamp_min(0)] = ups[0].abs().double()
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    bar = want.abs() * torch.finfo(dtype).eps / 2 + 4 * r * (size + hit) + tiny
+    assert ((grad.cpu().double() - want).abs() <= bar).all()
+
+
+def test_gradient_matches_differences(cuda_device):
+    """Central differences of the forward in steps of 2^-6: truncation h^2 / 6 of
+    third derivatives (at most 1 for log p and lse, (1 + |log p|) for H here) and
+    the forward's error over h."""
+    dev = cuda_device
+    z, t = _make(2, 40, torch.float32, spread=1.0)
+    x = z.to(dev).requires_grad_()
+    f = lambda y: (lambda r: (r.logprobs * 1.5 + r.entropy * 0.7 - r.lse * 0.4).sum())(ada.token_logprobs(y, t.to(dev)))
+    grad, = torch.autograd.grad(f(x), x)
+    h = 2.0 ** -6
+    for i in range(2):
+        for j in range(0, 40, 7):
+            e = torch.zeros_like(x)
+            e[i, j] = h
+            num = ((f(x + e) - f(x - e)) / (2 * h)).item()
+            assert abs(num - grad[i, j].item()) <= 8 * h * h / 6 * 4 + 2e-5 / h
+
+
+def test_partial_upstream_gradients(cuda_device):
+    """Only some outputs used; an entropy gradient reaches an ignored row, a log probability's does not."""
+    dev = cuda_device
+    z, t = _make(4, 300, torch.float32)
+    x = z.to(dev).requires_grad_()
+    zero = torch.zeros(4)
+    one = torch.ones(4)
+    for pick, ups in (("logprobs", (one, zero, zero)), ("entropy", (zero, one, zero)), ("lse", (zero, zero, one))):
+        grad, = torch.autograd.grad(getattr(ada.token_logprobs(x, t.to(dev)), pick).sum(), x)
+        assert (grad.cpu().double() - _grad64(z, t, *ups)).abs().max().item() <= 2e-6
+        assert (grad[1] == 0).all() == (pick == "logprobs")
+    r = ada.token_logprobs(x, t.to(dev), top_k=2)
+    assert not r.top_logprobs.requires_grad and not r.top_tokens.requires_grad
+    with torch.no_grad():
+        assert not ada.token_logprobs(x, t.to(dev)).logprobs.requires_grad
+
+
+def test_three_dimensional_gradient_of_a_shared_leaf(cuda_device):
+    dev = cuda_device
+    z, t = _make(12, 203, torch.bfloat16)
+    x = z.view(3, 4, 203).to(dev).requires_grad_()
+    r = ada.token_logprobs(x[:, :-1], t.view(3, 4)[:, 1:].to(dev))
+    r.logprobs.sum().backward()
+    zz, tt = z.view(3, 4, 203)[:, :-1].reshape(9, 203), t.view(3, 4)[:, 1:].reshape(9)
+    want = _grad64(zz, tt, torch.ones(9), torch.zeros(9), torch.zeros(9)).view(3, 3, 203)
+    got = x.grad.cpu().double()
+    assert (got[:, -1] == 0).all()
+    assert (got[:, :-1] - want).abs().max().item() <= 2.0 ** -9 + 1e-5
+
+
+def test_captured_forward_and_gradient(cuda_device):
+    """Two captured graphs and an eager call share nothing; a replay reads the new logits."""
+    dev = cuda_device
+    z, t = _make(8, 5000, torch.bfloat16)
+    zd, td = z.to(dev), t.to(dev)
+    ones = torch.ones(8, device=dev)
+
+    def step():
+        r = ada.token_logprobs(zd, td, top_k=4)
+        # the gradient's own entry, as a step captured without autograd uses it
+        m = zd.float().amax(-1)
+        stats = torch.stack([m, r.lse - m], 1)
+        return r, token_logprobs_backward(zd[None], td, stats, r.entropy, ones)
+
+    want = step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got = step()
+        graphs.append((gr, got))
+    z2, _ = _make(8, 5000, torch.bfloat16, seed=9)
+    for src in (z, z2, z):
+        zd.copy_(src)
+        want = step()
+        for gr, got in graphs:
+            gr.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(got[0], want[0]):
+                assert torch.equal(a, b)
+            assert torch.equal(got[1], want[1])
+
+
+def test_other_streams_repeat_the_bits(cuda_device):
+    dev = cuda_device
+    z, t = _make(20, 50257, torch.bfloat16)
+    zd, td = z.to(dev), t.to(dev)
+    a = ada.token_logprobs(zd, td, top_k=20)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        b = ada.token_logprobs(zd, td, top_k=20)
+    torch.cuda.synchronize()
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+def test_refusals(cuda_device):
+    dev = cuda_device
+    z, t = _make(4, 50, torch.float32)
+    z, t = z.to(dev), t.to(dev)
+    with pytest.raises(TypeError):
+        ada.token_logprobs(z.double(), t)
+    with pytest.raises(TypeError):
+        ada.token_logprobs(z, t.float())
+    with pytest.raises(ada.ShapeError):
+        ada.token_logprobs(z, t[:3])
+    with pytest.raises(ValueError):
+        ada.token_logprobs(z, t, top_k=65)
+    with pytest.raises(ValueError):
+        ada.token_logprobs(z, t, top_k=51)
+    with pytest.raises(RuntimeError):
+        ada.token_logprobs(z.cpu(), t)
+    with pytest.raises(RuntimeError):
+        ada.token_logprobs(z, t.cpu())
+    with pytest.raises(Exception):
+        ada.token_logprobs(z[:, :0], t)

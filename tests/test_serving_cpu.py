@@ -1,0 +1,196 @@
+"""Refusals of the serving operators that need no GPU: the C entry points
+answer bad arguments with a status code before they touch a device, the Python
+functions refuse host tensors, and the workspace sizes come from shapes alone."""
+
+import os
+
+import pytest
+import torch
+
+import adaattn_b200 as ada
+from adaattn_b200 import _lib
+from adaattn_b200.paged import _planes
+from serving_util import PoolModel, attend64, build_pool
+
+pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
+
+INVALID, SHAPE, DTYPE, LAYOUT, WORKSPACE, UNSUPPORTED = -1, -2, -3, -5, -8, -9
+T = _lib.tensor
+
+
+def _attn(q=None, k=None, v=None, table=None, lens=None, seqs=None, mask=None, ks=None, vs=None, out=None, ws=0):
+    q = torch.zeros(2, 4, 64) if q is None else q
+    k = torch.zeros(5, 2, 16, 64) if k is None else k
+    v = torch.zeros_like(k) if v is None else v
+    table = torch.zeros(2, 3, dtype=torch.int32) if table is None else table
+    lens = torch.zeros(table.shape[0], dtype=torch.int32) if lens is None else lens
+    out = torch.zeros_like(q) if out is None else out
+    o = lambda t: None if t is None else T(t)
+    buf = torch.zeros(max(ws, 1), dtype=torch.uint8)
+    return _lib.load().ada_paged_attn(T(q), T(k), T(v), T(table), T(lens), o(seqs), o(mask), o(ks), o(vs), 0.125, T(out),
+                                      None, buf.data_ptr() if ws else None, ws, None)
+
+
+def test_attention_refuses_before_any_device_work():
+    z = torch.zeros
+    assert _lib.load().ada_paged_attn(None, None, None, None, None, None, None, None, None, 1.0, None, None, None, 0,
+                                      None) == INVALID
+    assert _attn() == WORKSPACE and _attn(ws=64) == WORKSPACE
+    assert _attn(q=z(2, 4, 2, 64)) == SHAPE
+    assert _attn(q=z(2, 3, 64)) == SHAPE                       # 3 heads over 2
+    assert _attn(q=z(2, 4, 64, dtype=torch.float64)) == DTYPE
+    assert _attn(q=z(2, 4, 64, dtype=torch.float16)) == DTYPE  # pages are fp32
+    assert _attn(q=z(2, 4, 32)) == SHAPE
+    assert _attn(q=z(2, 4, 64), out=z(2, 4, 63)) == SHAPE
+    assert _attn(q=z(2, 64, 4).transpose(1, 2)) == LAYOUT
+    assert _attn(q=z(2, 4, 256), k=z(5, 2, 16, 256)) == UNSUPPORTED
+    assert _attn(k=z(5, 2, 0, 64)) == UNSUPPORTED
+    assert _attn(k=z(5, 2, 16, 64), v=z(5, 2, 8, 64)) == SHAPE
+    assert _attn(k=z(5, 2, 16, 64), v=z(5, 2, 16, 64, dtype=torch.float16)) == DTYPE
+    assert _attn(table=z(2, 3, dtype=torch.int64)) == DTYPE
+    assert _attn(table=z(3, 3, dtype=torch.int32)) == SHAPE    # a row per sequence unless picked
+    assert _attn(lens=z(3, dtype=torch.int32)) == SHAPE
+    assert _attn(seqs=z(3, dtype=torch.int32)) == SHAPE
+    assert _attn(seqs=z(2, dtype=torch.int64)) == DTYPE
+    assert _attn(mask=torch.ones(3, 40, dtype=torch.bool)) == SHAPE
+    assert _attn(mask=torch.ones(2, 40, dtype=torch.int32)) == DTYPE
+    assert _attn(ks=torch.ones(2)) == UNSUPPORTED              # scales go with 8-bit pages
+    k8 = z(5, 2, 16, 64).to(torch.float8_e4m3fn)
+    assert _attn(k=k8, ks=torch.ones(3)) == SHAPE
+    assert _attn(k=k8, ks=torch.ones(2, dtype=torch.float64)) == DTYPE
+    big = z(1, 4, 64).expand(5000, 4, 64)
+    assert _attn(q=big, table=z(5000, 1, dtype=torch.int32), out=big) == UNSUPPORTED
+
+
+def test_workspaces_come_from_shapes():
+    lib = _lib.load()
+    assert lib.ada_paged_attn_workspace_bytes(1, 32, 8, 128) > 0
+    assert lib.ada_paged_attn_workspace_bytes(1, 3, 2, 128) == 0
+    assert lib.ada_paged_attn_workspace_bytes(5000, 8, 8, 128) == 0
+    assert lib.ada_paged_attn_workspace_bytes(1, 8, 8, 129) == 0
+    a, b = lib.ada_pages_workspace_bytes(100, 10, 5), lib.ada_pages_workspace_bytes(1000, 10, 5)
+    assert 0 < a < b and lib.ada_pages_workspace_bytes(-1, 1, 1) == 0
+
+
+def _append(k=None, pages=None, table=None, lens=None, new=None, seqs=None, ks=None, v=None):
+    k = torch.zeros(2, 2, 3, 64) if k is None else k
+    pages = torch.zeros(5, 2, 16, 64) if pages is None else pages
+    table = torch.zeros(2, 3, dtype=torch.int32) if table is None else table
+    lens = torch.zeros(table.shape[0], dtype=torch.int32) if lens is None else lens
+    o = lambda t: None if t is None else T(t)
+    return _lib.load().ada_paged_append(T(k), T(k if v is None else v), T(pages), T(pages), T(table), T(lens), o(new),
+                                        o(seqs), o(ks), None, None)
+
+
+def test_append_refuses_before_any_device_work():
+    z = torch.zeros
+    assert _lib.load().ada_paged_append(*[None] * 11) == INVALID
+    assert _append(k=z(2, 2, 64)) == SHAPE
+    assert _append(k=z(2, 3, 3, 64)) == SHAPE
+    assert _append(v=z(2, 2, 4, 64)) == SHAPE
+    assert _append(k=z(2, 2, 3, 64, dtype=torch.bfloat16)) == DTYPE
+    assert _append(k=z(2, 2, 64, 3).transpose(2, 3)) == LAYOUT
+    assert _append(new=z(1, dtype=torch.int32)) == SHAPE
+    assert _append(new=z(2, dtype=torch.int64)) == DTYPE
+    assert _append(table=z(3, 3, dtype=torch.int32)) == SHAPE
+    assert _append(ks=torch.ones(2)) == UNSUPPORTED
+    assert _append(k=z(0, 2, 3, 64), table=z(0, 3, dtype=torch.int32)) == 0
+
+
+def test_page_operations_refuse_before_any_device_work():
+    lib, i32 = _lib.load(), torch.int32
+    table, lens, refs = torch.zeros(4, 3, dtype=i32), torch.zeros(4, dtype=i32), torch.zeros(7, dtype=i32)
+    one, two = torch.zeros(1, dtype=i32), torch.zeros(2, dtype=i32)
+    data = torch.zeros(2, 7, 2, 16, 8)
+    pool = (T(table), T(lens), T(refs))
+    assert lib.ada_pages_free(None, None, None, 16, None, None) == INVALID
+    assert lib.ada_pages_free(*pool, 0, T(one), None) == UNSUPPORTED
+    assert lib.ada_pages_free(*pool, 70000, T(one), None) == UNSUPPORTED
+    assert lib.ada_pages_free(T(table.long()), T(lens), T(refs), 16, T(one), None) == DTYPE
+    assert lib.ada_pages_free(T(table), T(lens[:3]), T(refs), 16, T(one), None) == SHAPE
+    assert lib.ada_pages_free(T(table[:, ::2]), T(lens), T(refs), 16, T(one), None) == LAYOUT
+    assert lib.ada_pages_free(T(table[:1].expand(4, 3)), T(lens), T(refs), 16, T(one), None) == LAYOUT
+    assert lib.ada_pages_free(*pool, 16, T(one.float()), None) == DTYPE
+    assert lib.ada_pages_fork(*pool, 16, T(one), T(two), None) == SHAPE
+    assert lib.ada_pages_fork(*pool, 16, T(one[:0]), T(one[:0]), None) == 0
+    p = _planes(data)
+    assert lib.ada_pages_reserve(p, *pool, 16, T(one), T(two), T(one), None, 0, None) == SHAPE
+    assert lib.ada_pages_reserve(p, *pool, 16, T(one), T(one), T(one), None, 0, None) == WORKSPACE
+    assert lib.ada_pages_reserve(_planes(data[:, :5]), *pool, 16, T(one), T(one), T(one), None, 0, None) == SHAPE
+    assert lib.ada_pages_copy(p, *pool, 16, T(one), T(one), T(two), None, 0, None) == SHAPE
+    assert lib.ada_pages_compact(p, *pool, 16, T(two), None, 0, None) == SHAPE
+    assert lib.ada_pages_compact(_planes(data.expand(2, 7, 2, 16, 8)[:1].expand(2, 7, 2, 16, 8)), *pool, 16, T(one),
+                                 None, 0, None) == LAYOUT
+    with pytest.raises(ada.ShapeError):
+        _planes(data.transpose(3, 4))
+
+
+def test_scores_refuse_before_any_device_work():
+    lib = _lib.load()
+    z, t = torch.zeros(1, 3, 10), torch.zeros(3, dtype=torch.int64)
+    outs = [torch.zeros(30) for _ in range(6)]
+    p = [o.data_ptr() for o in outs]
+
+    def call(z=z, t=t, k=0, nulls=False):
+        a = [None] * 6 if nulls else p
+        return lib.ada_token_logprobs(T(z), T(t), -100, k, *a, None)
+
+    assert lib.ada_token_logprobs(None, None, -100, 0, *[None] * 6, None) == INVALID
+    assert call(z=z[0]) == SHAPE and call(t=t[:2]) == SHAPE
+    assert call(z=z.double()) == DTYPE and call(t=t.float()) == DTYPE
+    assert call(z=z.transpose(1, 2)) in (SHAPE, LAYOUT)
+    assert call(k=65) == UNSUPPORTED and call(k=-1) == UNSUPPORTED and call(k=11) == SHAPE
+    assert call(z=z[:, :, :0]) == UNSUPPORTED
+    assert call(nulls=True) == INVALID
+    assert call(z=z[:, :0], t=t[:0]) == 0
+    grad = torch.zeros(1, 3, 9)
+    assert lib.ada_token_logprobs_bwd(T(z), T(t), -100, p[0], p[1], None, None, None, T(grad), None) == SHAPE
+    assert lib.ada_token_logprobs_bwd(T(z), T(t), -100, p[0], p[1], None, None, None, T(z.half()), None) == DTYPE
+    assert lib.ada_token_logprobs_bwd(T(z), T(t), -100, None, p[1], None, None, None, T(z), None) == INVALID
+
+
+def test_host_tensors_are_refused():
+    i32 = torch.int32
+    table, lens, refs = torch.zeros(2, 3, dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(5, dtype=i32)
+    pages, ids = torch.zeros(5, 2, 16, 64), torch.zeros(1, dtype=i32)
+    for call in (lambda: ada.paged_attention(torch.zeros(2, 4, 64), pages, pages, table, lens),
+                 lambda: ada.paged_append(torch.zeros(2, 2, 1, 64), torch.zeros(2, 2, 1, 64), pages, pages, table, lens),
+                 lambda: ada.reserve_pages(pages[None], table, lens, refs, ids, ids),
+                 lambda: ada.fork_pages(table, lens, refs, ids, ids, page_size=16),
+                 lambda: ada.copy_pages(pages[None], table, lens, refs, ids, ids),
+                 lambda: ada.free_pages(table, lens, refs, ids, page_size=16),
+                 lambda: ada.compact_pages(pages[None], table, lens, refs),
+                 lambda: ada.token_logprobs(torch.zeros(2, 5), torch.zeros(2, dtype=torch.int64))):
+        with pytest.raises(RuntimeError):
+            call()
+    with pytest.raises(ValueError):
+        ada.PagedKVCache(1, 0, 16, 2, 64, max_sequences=1, max_pages_per_sequence=1, device="cpu")
+    with pytest.raises(TypeError):
+        ada.PagedKVCache(1, 4, 16, 2, 64, max_sequences=1, max_pages_per_sequence=1, device="cpu", dtype=torch.float64)
+    with pytest.raises(TypeError):
+        ada.PagedKVCache(1, 4, 16, 2, 64, max_sequences=1, max_pages_per_sequence=1, device="cpu",
+                         k_scale=torch.ones(1, 2))
+    c = ada.PagedKVCache(2, 4, 16, 2, 64, max_sequences=1, max_pages_per_sequence=1, device="cpu")
+    assert c.keys(1).data_ptr() != c.values(1).data_ptr() and c.keys(0).shape == (4, 2, 16, 64)
+    with pytest.raises(IndexError):
+        c.keys(2)
+
+
+def test_the_references_themselves():
+    """The model of the page operations and the 64-bit attention agree with hand-made answers."""
+    g = torch.Generator().manual_seed(0)
+    k, v, table, ln = build_pool([3], 2, 1, 4, torch.float32, g)
+    q = torch.zeros(1, 2, 4)
+    out, lse = attend64(q, k, v, table, ln, 1.0)
+    rows = torch.cat([v[table[0, 0], 0], v[table[0, 1], 0, :1]]).double()
+    assert torch.allclose(out[0, 1], rows.mean(0)) and abs(lse[0, 0].item() - 1.0986122886681098) < 1e-12
+    m = PoolModel(torch.tensor([[4, 1], [-1, -1], [-1, -1]], dtype=torch.int32), torch.tensor([3, 0, 0], dtype=torch.int32),
+                  torch.tensor([0, 1, 0, 0, 1], dtype=torch.int32), torch.arange(10.).view(1, 5, 2), 2)
+    m.fork([0], [1])
+    assert m.refs.tolist() == [0, 2, 0, 0, 2]
+    assert m.reserve([0, 1], [1, 1]) == [1, 1]          # 0 copies the part-full page, 1 keeps it
+    assert m.table.tolist() == [[4, 0], [4, 1], [-1, -1]] and m.refs.tolist() == [1, 1, 0, 0, 2]
+    assert m.data[0, 0].tolist() == m.data[0, 1].tolist()
+    assert m.compact() == 3 and m.table.tolist() == [[2, 0], [2, 1], [-1, -1]]
+    m.free([0, 1])
+    assert m.refs.sum() == 0
