@@ -306,6 +306,10 @@ int launch_attn_bwd(const BwdLaunch& L, cudaStream_t stream);
 
 // --- paged key-value cache --------------------------------------------------------
 struct PagedAttnLaunch {
+    CUtensorMap tk, tv;  // tensor-core path: pages [P, Hkv, page, D], chunk x (up to 128 bytes) boxes
+    int tc;              // 1: the tensor-core kernel serves the call
+    int stages;          // ring slots per warp, set by the launcher
+    int chunk;           // keys per box: the largest power of two up to 32 that divides the page
     const void* q;       // [B, H, D]
     const void* k;       // [P, Hkv, page, D]
     const void* v;

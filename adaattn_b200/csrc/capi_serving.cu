@@ -125,7 +125,44 @@ int check_scales(const AdaTensor* s, const char* name, int64_t heads, int kv_dty
 constexpr int64_t kMaxBatch = 4096;  // the tile prefix is kept in shared memory
 constexpr int kMaxCtas = 2 * 148;    // pieces that the workspace is sized for
 
-int heads_per_block(int64_t g) { return g <= 1 ? 1 : g <= 2 ? 2 : g <= 4 ? 4 : 8; }
+// Query heads per block: the tensor-core kernel takes 8 or 16 (its products'
+// narrow side), the CUDA-core kernel up to 8.
+int heads_per_block(int64_t g, bool tc) { return tc ? (g <= 8 ? 8 : 16) : g <= 1 ? 1 : g <= 2 ? 2 : g <= 4 ? 4 : 8; }
+
+// A tensor map over pages [P, Hkv, page, D] (innermost first: D, page, Hkv, P)
+// with boxes of `rows` keys x up to 128 bytes, swizzled over that width.
+int pages_map(CUtensorMap* map, const AdaTensor* t, int rows) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc;
+    int rc = tensor_map_encoder(&enc);
+    if (rc) return rc;
+    const int eb = elt_bytes(t->dtype);
+    const int64_t row = t->shape[3] * eb;
+    cuuint64_t dims[4], strides[3];
+    int64_t dense = row;
+    for (int i = 0; i < 4; ++i) dims[i] = static_cast<cuuint64_t>(t->shape[3 - i]);
+    for (int i = 0; i < 3; ++i) {
+        strides[i] = static_cast<cuuint64_t>(t->shape[2 - i] > 1 ? t->stride[2 - i] * eb : dense);
+        dense = static_cast<int64_t>(strides[i]) * t->shape[2 - i];
+    }
+    cuuint32_t box[4] = {static_cast<cuuint32_t>(std::min<int64_t>(row, 128) / eb), static_cast<cuuint32_t>(rows), 1, 1};
+    cuuint32_t es[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType dt = t->dtype == ADA_F16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                   : t->dtype == ADA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUresult r = enc(map, dt, 4, t->data, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           row >= 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ADA_ERR_LAYOUT, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return ADA_OK;
+}
+
+// Whether TMA can read the pages: rows on 16-byte boundaries, positive strides below 2^40 bytes.
+bool tma_pages(const AdaTensor* t, int eb) {
+    if (!rows_aligned(t, eb, 16) || t->shape[0] < 1) return false;
+    for (int i = 0; i < 3; ++i)
+        if (t->shape[i] > 1 && (t->stride[i] <= 0 || t->stride[i] * eb >= (int64_t(1) << 40))) return false;
+    return true;
+}
 
 // ---- page operations ---------------------------------------------------------------
 
@@ -254,7 +291,7 @@ extern "C" {
 size_t ada_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim) {
     if (batch < 0 || batch > kMaxBatch || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || head_dim > 128)
         return 0;
-    const size_t gb = static_cast<size_t>(heads_per_block(heads / kv_heads));
+    const size_t gb = static_cast<size_t>(heads_per_block(heads / kv_heads, true));
     return align256(static_cast<size_t>(batch + 1) * 4) + align256(kMaxCtas * 2 * gb * 2 * 4) +
            align256(kMaxCtas * 2 * gb * static_cast<size_t>(head_dim) * 4);
 }
@@ -331,13 +368,21 @@ int ada_paged_attn(const AdaTensor* q, const AdaTensor* k_pages, const AdaTensor
     L.H = static_cast<int>(H);
     L.D = static_cast<int>(D);
     L.G = static_cast<int>(H / Hkv);
-    L.GB = heads_per_block(L.G);
+    // The tensor-core kernel serves 16- and 8-bit pages that TMA can read with
+    // heads of 64 or 128 and a page of a multiple of 8 keys (a swizzle's rows).
+    L.tc = k_pages->dtype != ADA_F32 && q->dtype != ADA_F32 && (D == 64 || D == 128) && page % 8 == 0 &&
+           tma_pages(k_pages, eb) && tma_pages(v_pages, eb) && rows_aligned(q, 2, 4);
+    if (L.tc) {
+        L.chunk = static_cast<int>(std::min<int64_t>(32, page & -page));
+        if ((rc = pages_map(&L.tk, k_pages, L.chunk)) || (rc = pages_map(&L.tv, v_pages, L.chunk))) return rc;
+    }
+    L.GB = heads_per_block(L.G, L.tc != 0);
     L.HB = (L.G + L.GB - 1) / L.GB;
     L.U = Hkv * L.HB;
     if (B * L.U > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "too many heads");
     L.out = out->data;
     L.lse = lse;
-    L.n_cta = std::min(kMaxCtas, 2 * sms);
+    L.n_cta = std::min(kMaxCtas, L.tc ? sms : 2 * sms);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     L.pref = reinterpret_cast<int*>(ws);
     ws += align256(static_cast<size_t>(B + 1) * 4);

@@ -171,17 +171,20 @@ struct Left {
     int64_t t0, t1;
 };
 
+// Accumulators [GB][DP] and (m, l) [GB][2] of the block's warps and slots.
 struct Join {
-    float* acc;   // [kWarps][2][GB][DP]
-    float* ml;    // [kWarps][2][GB][2]
-    Left* left;   // [kWarps][2]
+    float* acc[2];   // of warp 0, by slot
+    int stride[2];   // floats from one warp's to the next one's
+    float* ml;       // [warps][2][GB][2]
+    Left* left;      // [warps][2]
+    __device__ float* part(int warp, int slot) const { return acc[slot] + warp * stride[slot]; }
 };
 
 // Joins the pieces that the block's warps left. A unit inside the block's own
 // piece [a, z) is finished; another goes to the workspace, slot 0 / 1 as above.
-template <int GB, int DP>
+template <int WARPS, int GB, int DP>
 __device__ void join_block(const PagedAttnLaunch& L, const Join& J, int64_t a, int64_t z) {
-    constexpr int NE = 2 * kWarps;
+    constexpr int NE = 2 * WARPS;
     int e = 0;
     while (e < NE) {
         if (!J.left[e].valid) {
@@ -195,7 +198,7 @@ __device__ void join_block(const PagedAttnLaunch& L, const Join& J, int64_t a, i
         const int heads = min(GB, (g + 1) * L.G - h0);
         const bool whole = x.t0 >= a && x.t1 <= z;
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (x.t0 < a ? 0 : 1);
-        for (int i = threadIdx.x; i < heads * DP; i += kThreads) {
+        for (int i = threadIdx.x; i < heads * DP; i += WARPS * 32) {
             const int h = i / DP, d = i - h * DP;
             float m = -INFINITY;
             for (int k = e; k < end; ++k)
@@ -206,7 +209,7 @@ __device__ void join_block(const PagedAttnLaunch& L, const Join& J, int64_t a, i
                 if (!J.left[k].valid) continue;
                 const float w = exp2f((J.ml[(k * GB + h) * 2] - ref) * kLog2e);
                 l += w * J.ml[(k * GB + h) * 2 + 1];
-                acc += w * J.acc[(k * GB + h) * DP + d];
+                acc += w * J.part(k >> 1, k & 1)[h * DP + d];
             }
             if (whole) {
                 if (d < L.D) store_out(L, x.b, h0 + h, d, l == 0.f ? 0.f : acc / l * value_scale(L, g));
@@ -223,44 +226,65 @@ __device__ void join_block(const PagedAttnLaunch& L, const Join& J, int64_t a, i
     }
 }
 
-// Joins what CTAs left of each unit that spans several, and writes the units of empty sequences.
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttnLaunch L) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t unit = blockIdx.x;
-    const int b = static_cast<int>(unit / L.U), u = static_cast<int>(unit % L.U);
-    const int g = u / L.HB, h0 = g * L.G + (u % L.HB) * L.GB;
-    const int heads = min(L.GB, (g + 1) * L.G - h0);
-    const int first = L.pref[b], n = L.pref[b + 1] - first;
-    if (n == 0) {
-        for (int i = threadIdx.x; i < heads * L.D; i += kThreads) store_out(L, b, h0 + i / L.D, i % L.D, 0.f);
-        if (L.lse != nullptr && threadIdx.x < heads) L.lse[static_cast<int64_t>(b) * L.H + h0 + threadIdx.x] = -INFINITY;
-        return;
+// The outputs of sequences without keys, shared out over the grid.
+__device__ void write_empty(const PagedAttnLaunch& L, const int* pref) {
+    for (int b = blockIdx.x; b < L.B; b += gridDim.x) {
+        if (pref[b + 1] != pref[b]) continue;
+        for (int i = threadIdx.x; i < L.H * L.D; i += blockDim.x) store_out(L, b, i / L.D, i % L.D, 0.f);
+        if (L.lse != nullptr)
+            for (int h = threadIdx.x; h < L.H; h += blockDim.x) L.lse[static_cast<int64_t>(b) * L.H + h] = -INFINITY;
     }
+}
+
+// Joins what CTAs left of a unit that spans several: block (c, h) serves head
+// h of the unit that goes on from CTA c's piece into the next one, when it
+// began in c's. Its partial sums are one per CTA: c's in slot 1, the others'
+// in slot 0. The weights of up to 512 parts are worked out side by side.
+constexpr int kJoinThreads = 128;
+constexpr int kMaxParts = 512;
+
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttnLaunch L) {
+    __shared__ float s_w[kMaxParts];
+    __shared__ float s_red[2][kJoinThreads / 32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t T = static_cast<int64_t>(L.pref[L.B]) * L.U;
     const int64_t nc = pieces(T, L.n_cta);
-    const int64_t t0 = static_cast<int64_t>(first) * L.U + static_cast<int64_t>(u) * n;
-    const int64_t c0 = piece_of(t0, T, nc), c1 = piece_of(t0 + n - 1, T, nc);
-    if (c0 == c1) return;
-    const int64_t slot0 = c0 * 2 + 1;  // the unit begins in c0's piece; later CTAs begin inside the unit: slot 0
-    for (int i = threadIdx.x; i < heads * L.D; i += kThreads) {
-        const int h = i / L.D, d = i - h * L.D;
-        float m = -INFINITY;
-        for (int64_t c = c0; c <= c1; ++c) {
-            const int64_t s = c == c0 ? slot0 : c * 2;
-            m = fmaxf(m, L.part_ml[(s * L.GB + h) * 2]);
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float l = 0.f, acc = 0.f;
-#pragma unroll 4
-        for (int64_t c = c0; c <= c1; ++c) {
-            const int64_t s = c == c0 ? slot0 : c * 2;
-            const float w = exp2f((L.part_ml[(s * L.GB + h) * 2] - ref) * kLog2e);
-            l += w * L.part_ml[(s * L.GB + h) * 2 + 1];
-            acc += w * L.part_acc[(s * L.GB + h) * L.D + d];
-        }
-        store_out(L, b, h0 + h, d, l == 0.f ? 0.f : acc / l * value_scale(L, g));
-        if (d == 0 && L.lse != nullptr) L.lse[static_cast<int64_t>(b) * L.H + h0 + h] = m + logf(l);
+    const int64_t c0 = blockIdx.x;
+    const int h = blockIdx.y, tid = threadIdx.x;
+    if (c0 + 1 >= nc) return;
+    const int64_t edge = piece_start(c0 + 1, T, nc);
+    const Unit x = unit_at(L, L.pref, edge);
+    if (x.t0 == edge || piece_of(x.t0, T, nc) != c0) return;
+    const int g = x.u / L.HB, h0 = g * L.G + (x.u % L.HB) * L.GB;
+    if (h >= min(L.GB, (g + 1) * L.G - h0)) return;
+    const int n = static_cast<int>(piece_of(x.t1 - 1, T, nc) - c0 + 1);
+    auto slot = [&](int i) { return (c0 + i) * 2 + (i == 0 ? 1 : 0); };
+    float m = -INFINITY;
+    for (int i = tid; i < n; i += kJoinThreads) m = fmaxf(m, L.part_ml[(slot(i) * L.GB + h) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((tid & 31) == 0) s_red[0][tid >> 5] = m;
+    __syncthreads();
+    for (int w = 0; w < kJoinThreads / 32; ++w) m = fmaxf(m, s_red[0][w]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int i = tid; i < n; i += kJoinThreads) {
+        const float w = exp2f((L.part_ml[(slot(i) * L.GB + h) * 2] - ref) * kLog2e);
+        s_w[i] = w;
+        l += w * L.part_ml[(slot(i) * L.GB + h) * 2 + 1];
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if ((tid & 31) == 0) s_red[1][tid >> 5] = l;
+    __syncthreads();
+    l = 0.f;
+    for (int w = 0; w < kJoinThreads / 32; ++w) l += s_red[1][w];
+    if (tid == 0 && L.lse != nullptr) L.lse[static_cast<int64_t>(x.b) * L.H + h0 + h] = m + logf(l);
+    if (tid >= L.D) return;
+    float acc = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) acc = fmaf(s_w[i], L.part_acc[(slot(i) * L.GB + h) * L.D + tid], acc);
+    store_out(L, x.b, h0 + h, tid, l == 0.f ? 0.f : acc / l * value_scale(L, g));
 }
 
 // ---- CUDA-core kernel: every type, head dim and layout ------------------------
@@ -296,8 +320,10 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const __grid_const
     __shared__ Left s_left[2 * kWarps];
     __shared__ int s_sums[kWarps];
     Join J;
-    J.acc = reinterpret_cast<float*>(smem);
-    J.ml = J.acc + 2 * kWarps * GB * DP;
+    J.acc[0] = reinterpret_cast<float*>(smem);
+    J.acc[1] = J.acc[0] + GB * DP;
+    J.stride[0] = J.stride[1] = 2 * GB * DP;
+    J.ml = J.acc[0] + 2 * kWarps * GB * DP;
     J.left = s_left;
     int* pref = reinterpret_cast<int*>(J.ml + 2 * kWarps * GB * 2);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -306,6 +332,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const __grid_const
     tile_prefix(L, pref, s_sums);
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= L.B; b += kThreads) L.pref[b] = pref[b];
+    write_empty(L, pref);
     const int64_t T = static_cast<int64_t>(pref[L.B]) * L.U;
     const int64_t nc = pieces(T, L.n_cta);
     if (static_cast<int64_t>(blockIdx.x) >= nc) return;
@@ -423,7 +450,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const __grid_const
             }
         }
         const bool whole = x.t0 >= a && x.t1 <= z;
-        const int slot = warp * 2 + (x.t0 < a ? 0 : 1);
+        const int side = x.t0 < a ? 0 : 1, slot = warp * 2 + side;
         const float vs = value_scale(L, g);
 #pragma unroll
         for (int h = 0; h < GB; ++h) {
@@ -437,7 +464,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const __grid_const
                         if (c0 + i < L.D) store_out(L, x.b, h0 + h, c0 + i, lh == 0.f ? 0.f : o[i] / lh * vs);
                 if (lane == 0 && L.lse != nullptr) L.lse[static_cast<int64_t>(x.b) * L.H + h0 + h] = mh + logf(lh);
             } else {
-                if (kg == 0) *reinterpret_cast<float4*>(J.acc + (slot * GB + h) * DP + c0) = acc[h];
+                if (kg == 0) *reinterpret_cast<float4*>(J.part(warp, side) + h * DP + c0) = acc[h];
                 if (lane == 0) {
                     J.ml[(slot * GB + h) * 2] = mh;
                     J.ml[(slot * GB + h) * 2 + 1] = lh;
@@ -448,7 +475,7 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const __grid_const
         __syncwarp();
     }
     __syncthreads();
-    join_block<GB, DP>(L, J, ca, cz);
+    join_block<kWarps, GB, DP>(L, J, ca, cz);
 }
 
 template <int DT, int GB, int LPK, bool VEC>
@@ -479,22 +506,517 @@ int launch_simt_gb(const PagedAttnLaunch& L, cudaStream_t stream) {
     }
 }
 
+
+// ---- tensor-core kernel: 16-bit and 8-bit pages, head dims 64 and 128 ----------
+//
+// Query heads of a group are few (8, or 16 with NT = 2), so they take the
+// narrow side of the warp-level products: S^T = K q^T is 16 keys x 8 heads and
+// O^T += V^T P^T is 16 elements x 8 heads per instruction (m16n8k16), where
+// padding the heads to a 128-row tile would leave most of it empty. Scores
+// come out with a key per row; an 8 x 8 transpose in registers (movmatrix)
+// turns P into the next product's operand. P enters as two 16-bit parts
+// (hi + lo, 16 bits for bf16 and 22 for fp16), so that only the output is
+// rounded. 8-bit pages become fp16 operands in registers: E4M3 values are fp16
+// values, q is scaled into fp16's range by a power of two per head. The order
+// of elements within a head is free as long as K and q agree on it, and V's
+// with the output, so 4 consecutive bytes of a row serve two k positions.
+//
+// Every warp runs alone: it requests its own tiles by TMA, STAGES ahead (also
+// across units), into its own ring, and no barrier is shared between warps
+// until the join at the end. One CTA per SM with 192 KB of tiles in flight.
+template <int KIND, int D, int NT>  // KIND: 0 bf16, 1 fp16, 2 E4M3
+struct TcCfg {
+    static constexpr int EB = KIND == 2 ? 1 : 2;
+    static constexpr int RB = D * EB < 128 ? D * EB : 128;   // bytes of a box row, and of its swizzle
+    static constexpr int NBOX = D * EB / RB;
+    static constexpr int HALF = kTile * D * EB;              // K or V bytes of a tile
+    static constexpr int TILE = 2 * HALF;
+    static constexpr int WARPS = TILE >= 16384 ? 4 : 8;
+    static constexpr int STAGES = TILE >= 8192 ? 3 : 6;      // at most; fewer when the rest needs the space
+    static constexpr int GB = 8 * NT;
+    static constexpr int PART = GB * D;                      // floats a warp leaves per slot
+    // beside the ring: slot 0 of the join (slot 1 lies in the drained ring) and (m, l)
+    static constexpr int BESIDE = WARPS * (PART * 4 + 2 * GB * 2 * 4);
+};
+
+template <int KIND>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (KIND == 0)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// Four E4M3 bytes as two fp16 pairs.
+__device__ __forceinline__ void e4m3_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+}
+// p as a 16-bit pair hi + lo of the operand type.
+template <int KIND>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    if constexpr (KIND == 0) {
+        hi = pack_bf16x2(x, y);
+        lo = pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
+    } else {
+        hi = pack_f16x2(x, y);
+        float a, b;
+        unpack_f16x2(hi, a, b);
+        lo = pack_f16x2(x - a, y - b);
+    }
+}
+
+template <int KIND, int D, int NT>
+__global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
+    paged_tc_kernel(const __grid_constant__ PagedAttnLaunch L) {
+    using C = TcCfg<KIND, D, NT>;
+    constexpr int EB = C::EB, RB = C::RB, W = C::WARPS, SMAX = C::STAGES, GB = C::GB;
+    const int S = L.stages, ring_bytes = S * C::TILE;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ Left s_left[2 * W];
+    __shared__ int s_sums[W];
+    __shared__ __align__(8) uint64_t s_full[W * SMAX];
+    __shared__ uint32_t s_ok[W * SMAX];
+    __shared__ int s_abort;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint8_t* ring = smem + warp * ring_bytes;
+    Join J;
+    J.acc[0] = reinterpret_cast<float*>(smem + W * ring_bytes);
+    J.stride[0] = C::PART;
+    J.acc[1] = reinterpret_cast<float*>(smem);
+    J.stride[1] = ring_bytes / 4;
+    J.ml = J.acc[0] + W * C::PART;
+    J.left = s_left;
+    int* pref = reinterpret_cast<int*>(J.ml + W * 2 * GB * 2);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x < 2 * W) s_left[threadIdx.x].valid = 0;
+    if (threadIdx.x == 0) s_abort = 0;
+    if (lane == 0)
+        for (int i = 0; i < S; ++i) mbar_init(smem_u32(&s_full[warp * SMAX + i]), 1);
+    fence_mbar_init();
+    tile_prefix(L, pref, s_sums);
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= L.B; b += W * 32) L.pref[b] = pref[b];
+    write_empty(L, pref);
+    const int64_t T = static_cast<int64_t>(pref[L.B]) * L.U;
+    const int64_t nc = pieces(T, L.n_cta);
+    if (static_cast<int64_t>(blockIdx.x) >= nc) return;
+    const int64_t ca = piece_start(blockIdx.x, T, nc), cz = piece_start(blockIdx.x + 1, T, nc);
+    const int64_t a = ca + (cz - ca) * warp / W, z = ca + (cz - ca) * (warp + 1) / W;
+
+    // launch fields that the loop uses (barrier asm would have them reloaded)
+    const int page = L.page, CK = L.chunk, G = L.G, HB = L.HB, mask_len = static_cast<int>(L.mask_len);
+    const int64_t P = L.P, table_ld = L.table_ld;
+    const int32_t* table = L.table;
+    const void* mask = L.mask.data;
+    const int mask_type = L.mask.dtype;
+    unsigned int* status = L.status;
+    const uint64_t limit = L.timeout_ns;
+    const uint32_t bar0 = smem_u32(&s_full[warp * SMAX]), ring0 = smem_u32(ring);
+    volatile int* abort_flag = &s_abort;
+
+    // ---- requests: lane i issues box i of a tile (chunk, K or V, half of the row)
+    const int nch = kTile / CK;
+    const int my_chunk = lane % nch, my_v = (lane / nch) & 1, my_box = lane / (2 * nch);
+    const bool issues = my_box < C::NBOX;
+    int64_t pt = a, prow = 0;
+    Unit px{};
+    int plen = 0, pid = -1;
+    auto look_up = [&]() {  // unit of tile pt and this lane's page of it
+        pid = -1;
+        if (pt >= z) return;
+        if (pt == a || pt == px.t1) {
+            px = unit_at(L, pref, pt);
+            prow = table_row(L, px.b);
+            plen = seq_length(L, px.b);
+        }
+        const int key = static_cast<int>(pt - px.t0) * kTile + my_chunk * CK;
+        if (issues && key < plen) pid = table[prow * table_ld + key / page];
+    };
+    auto request = [&](int slot) {
+        const int key = static_cast<int>(pt - px.t0) * kTile + my_chunk * CK;
+        bool ok = issues && key < plen;
+        if (ok && (pid < 0 || pid >= P)) {
+            record_error(status, ADA_ERR_INVALID);
+            ok = false;
+        }
+        const uint32_t who = __ballot_sync(0xffffffffu, ok);
+        const uint32_t bar = bar0 + slot * 8;
+        if (lane == 0) {
+            s_ok[warp * SMAX + slot] = who;  // lanes 0 .. nch - 1 are the chunks
+            mbar_arrive_expect_tx(bar, __popc(who) * CK * RB);
+        }
+        __syncwarp();
+        if (ok)
+            tma_load_4d(ring0 + slot * C::TILE + my_v * C::HALF + my_box * (kTile * RB) + my_chunk * CK * RB,
+                        my_v ? &L.tv : &L.tk, bar, my_box * (RB / EB), key % page, px.u / HB, pid);
+        ++pt;
+        look_up();
+    };
+    look_up();
+    for (int i = 0; i < S && pt < z; ++i) request(i);
+
+    // ---- this lane's part of every fragment: keys / elements g and g + 8, heads 2 t and 2 t + 1
+    const int fg = lane >> 2, ft = lane & 3;
+    // ldmatrix row addresses: K rows (lane & 15), 16-byte column lane >> 4; V rows and columns as the kind needs
+    const int l7 = lane & 7;
+    auto swz = [](int row, int col) { return RB == 128 ? (col ^ (row & 7)) : (col ^ ((row >> 1) & 3)); };
+    const uint32_t k_row = static_cast<uint32_t>((lane & 15) * RB);
+    const int k_col = lane >> 4;
+    const int v_key = KIND == 2 ? (lane & 15) : ((lane >> 4) * 8 + l7);
+    const int v_col = KIND == 2 ? (lane >> 4) : ((lane >> 3) & 1);
+
+    int64_t t = a;
+    int slot = 0;             // the ring's slot of tile t and the parity of its barrier
+    uint32_t parity = 0;
+    bool alive = true;
+    while (t < z && alive) {
+        const Unit x = unit_at(L, pref, t);
+        const int64_t tz = x.t1 < z ? x.t1 : z;
+        const int g = x.u / HB, h0 = g * G + (x.u % HB) * GB;
+        const int heads = min(GB, (g + 1) * G - h0);
+        const int len = seq_length(L, x.b);
+        const int64_t mrow = x.b * L.mask.s[0], mcol = L.mask.s[1];
+        // q^T: element pairs of head fg (of each tile of 8 heads)
+        uint32_t qf[D / 16][NT][2];
+        float qs[NT][2];
+        {
+            const float base = L.scale * (L.k_scale != nullptr ? L.k_scale[g] : 1.f);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const bool on = n * 8 + fg < heads;
+                const uint32_t* qr = reinterpret_cast<const uint32_t*>(
+                    static_cast<const uint16_t*>(L.q) + x.b * L.qs[0] + (h0 + n * 8 + fg) * L.qs[1]);
+                if constexpr (KIND != 2) {
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s) {
+                        qf[s][n][0] = on ? qr[s * 8 + ft] : 0u;
+                        qf[s][n][1] = on ? qr[s * 8 + ft + 4] : 0u;
+                    }
+                    qs[n][0] = qs[n][1] = base;
+                } else {
+                    float top = 0.f;
+                    const bool half = L.q_dtype == ADA_F16;
+                    auto pair = [&](uint32_t w, float& lo, float& hi) {
+                        if (half) {
+                            unpack_f16x2(w, lo, hi);
+                        } else {
+                            lo = __uint_as_float(w << 16);
+                            hi = __uint_as_float(w & 0xFFFF0000u);
+                        }
+                    };
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            qf[s][n][i] = on ? qr[s * 8 + 2 * ft + i] : 0u;
+                            float lo, hi;
+                            pair(qf[s][n][i], lo, hi);
+                            top = fmaxf(top, fmaxf(fabsf(lo), fabsf(hi)));
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    // 2^-e with max |q| 2^-e in [1, 2); none for 0, infinity and what 2^-e does not fit
+                    const uint32_t e = (__float_as_uint(top) >> 23) & 0xFFu;
+                    const bool fits = e >= 1 && e <= 253;
+                    const float down = fits ? __uint_as_float((254u - e) << 23) : 1.f;
+                    const float up = fits ? __uint_as_float(e << 23) : 1.f;
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float lo, hi;
+                            pair(qf[s][n][i], lo, hi);
+                            qf[s][n][i] = pack_f16x2(lo * down, hi * down);
+                        }
+                    qs[n][0] = base * __shfl_sync(0xffffffffu, up, 8 * ft);
+                    qs[n][1] = base * __shfl_sync(0xffffffffu, up, 8 * ft + 4);
+                }
+            }
+        }
+        float o[D / 16][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+        }
+        for (; t < tz; ++t) {
+            const int key0 = static_cast<int>(t - x.t0) * kTile;
+            // lane i: key i's mask
+            bool open = key0 + lane < len;
+            float add = 0.f;
+            if (mask != nullptr && open && key0 + lane < mask_len) {
+                const float mv = load_as_f32(mask, mrow + (key0 + lane) * mcol, mask_type);
+                if (mask_type == ADA_BOOL) {
+                    open = mv != 0.f;
+                } else {
+                    open = mv != -INFINITY;
+                    add = open ? mv : 0.f;
+                }
+            }
+            if (!mbar_wait(bar0 + slot * 8, parity, abort_flag, limit, status)) {
+                alive = false;
+                break;
+            }
+            open = open && ((s_ok[warp * SMAX + slot] >> (lane / CK)) & 1u);
+            const uint32_t vis = __ballot_sync(0xffffffffu, open);
+            const uint32_t kb = ring0 + slot * C::TILE, vb = kb + C::HALF;
+            // S^T = K q^T
+            float c[2][NT][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[r][n][e] = 0.f;
+            if constexpr (KIND != 2) {
+#pragma unroll
+                for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        uint32_t f[4];
+                        const int col = (s & 3) * 2 + k_col;
+                        ldsm4(f, kb + (s >> 2) * (kTile * RB) + r * 16 * RB + k_row + swz(lane & 15, col) * 16);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16816<KIND>(c[r][n], f, qf[s][n][0], qf[s][n][1]);
+                    }
+            } else {
+#pragma unroll
+                for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        uint32_t w[4], f0[4], f1[4];
+                        ldsm4(w, kb + r * 16 * RB + k_row + swz(lane & 15, 2 * s + k_col) * 16);
+                        e4m3_to_f16(w[0], f0[0], f0[2]);
+                        e4m3_to_f16(w[1], f0[1], f0[3]);
+                        e4m3_to_f16(w[2], f1[0], f1[2]);
+                        e4m3_to_f16(w[3], f1[1], f1[3]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma_16816<KIND>(c[r][n], f0, qf[2 * s][n][0], qf[2 * s][n][1]);
+                            mma_16816<KIND>(c[r][n], f1, qf[2 * s + 1][n][0], qf[2 * s + 1][n][1]);
+                        }
+                    }
+            }
+            // scores, their maximum over the tile, probabilities
+            float av[2][2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    av[r][j] = mask != nullptr ? __shfl_sync(0xffffffffu, add, r * 16 + j * 8 + fg) : 0.f;
+            bool moved = false;
+            uint32_t ph[2][NT][2], pl[2][NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float ref[2], alpha[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float sc = fmaf(c[r][n][2 * j + e], qs[n][e], av[r][j]);
+                            c[r][n][2 * j + e] = ((vis >> (r * 16 + j * 8 + fg)) & 1u) ? sc : -INFINITY;
+                            top = fmaxf(top, c[r][n][2 * j + e]);
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float mn = fmaxf(m[n][e], top);
+                    ref[e] = mn == -INFINITY ? 0.f : mn;
+                    moved = moved || mn != m[n][e];
+                    alpha[e] = fast_exp2((m[n][e] - ref[e]) * kLog2e);
+                    m[n][e] = mn;
+                    l[n][e] *= alpha[e];
+                }
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float p0 = fast_exp2((c[r][n][2 * j] - ref[0]) * kLog2e);
+                        const float p1 = fast_exp2((c[r][n][2 * j + 1] - ref[1]) * kLog2e);
+                        l[n][0] += p0;
+                        l[n][1] += p1;
+                        uint32_t hi, lo;
+                        split2<KIND>(p0, p1, hi, lo);
+                        ph[r][n][j] = transpose8x8(hi);
+                        pl[r][n][j] = transpose8x8(lo);
+                    }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        o[i][n][0] *= alpha[0];
+                        o[i][n][1] *= alpha[1];
+                        o[i][n][2] *= alpha[0];
+                        o[i][n][3] *= alpha[1];
+                    }
+                }
+                moved = false;
+            }
+            // O^T += V^T P^T; a hidden key's values are zeroed, whatever they hold
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const uint32_t seen = (vis >> (r * 16)) & 0xFFFFu;
+                const uint32_t pair0 = (seen >> (2 * ft)) & 3u, pair1 = (seen >> (2 * ft + 8)) & 3u;
+                const uint32_t keep0 = (pair0 & 1u ? 0xFFFFu : 0u) | (pair0 & 2u ? 0xFFFF0000u : 0u);
+                const uint32_t keep1 = (pair1 & 1u ? 0xFFFFu : 0u) | (pair1 & 2u ? 0xFFFF0000u : 0u);
+                auto product = [&](int i, uint32_t (&f)[4]) {
+                    if (seen != 0xFFFFu) {
+                        f[0] &= keep0;
+                        f[1] &= keep0;
+                        f[2] &= keep1;
+                        f[3] &= keep1;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma_16816<KIND>(o[i][n], f, ph[r][n][0], ph[r][n][1]);
+                        mma_16816<KIND>(o[i][n], f, pl[r][n][0], pl[r][n][1]);
+                    }
+                };
+                if constexpr (KIND != 2) {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        uint32_t f[4];
+                        const int col = (i & 3) * 2 + v_col;
+                        ldsm4_t(f, vb + (i >> 2) * (kTile * RB) + (r * 16 + v_key) * RB + swz(v_key, col) * 16);
+                        product(i, f);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        uint32_t w[4], f0[4], f1[4];
+                        ldsm4_t(w, vb + (r * 16 + v_key) * RB + swz(v_key, 2 * i + v_col) * 16);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = __byte_perm(w[e], 0, 0x3120);
+                        e4m3_to_f16(w[0], f0[0], f0[1]);
+                        e4m3_to_f16(w[1], f0[2], f0[3]);
+                        e4m3_to_f16(w[2], f1[0], f1[1]);
+                        e4m3_to_f16(w[3], f1[2], f1[3]);
+                        product(2 * i, f0);
+                        product(2 * i + 1, f1);
+                    }
+                }
+            }
+            __syncwarp();  // the slot is read
+            if (pt < z) request(slot);
+            if (++slot == S) {
+                slot = 0;
+                parity ^= 1u;
+            }
+        }
+        if (!alive) break;
+        const bool whole = x.t0 >= a && x.t1 <= z;
+        const int side = x.t0 < a ? 0 : 1, left = warp * 2 + side;
+        float* part = J.part(warp, side);
+        const float vs = value_scale(L, g);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float sum = l[n][e];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int h = n * 8 + 2 * ft + e;
+                if (h >= heads) continue;
+                const float inv = whole ? (sum == 0.f ? 0.f : vs / sum) : 1.f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int d = KIND == 2 ? i * 16 + 2 * fg + j : i * 16 + fg + 8 * j;
+                        const float v = sum == 0.f ? 0.f : o[i][n][2 * j + e] * inv;
+                        if (whole) store_out(L, x.b, h0 + h, d, v);
+                        else part[h * D + d] = v;
+                    }
+                if (fg == 0) {
+                    if (whole) {
+                        if (L.lse != nullptr) L.lse[static_cast<int64_t>(x.b) * L.H + h0 + h] = m[n][e] + logf(sum);
+                    } else {
+                        J.ml[(left * GB + h) * 2] = m[n][e];
+                        J.ml[(left * GB + h) * 2 + 1] = sum;
+                    }
+                }
+            }
+        if (!whole && lane == 0) s_left[left] = Left{1, x.b, x.u, x.t0, x.t1};
+        __syncwarp();
+    }
+    if (!alive) {  // a wait ran out (recorded): the tiles still requested are awaited, then the block gives up
+        for (; t < pt; ++t) {
+            const uint64_t t0 = globaltimer_ns();
+            while (!mbar_try_wait(bar0 + slot * 8, parity) && globaltimer_ns() - t0 < limit) {}
+            if (++slot == S) {
+                slot = 0;
+                parity ^= 1u;
+            }
+        }
+    }
+    __syncthreads();
+    if (s_abort) return;
+    join_block<W, GB, D>(L, J, ca, cz);
+}
+
+template <int KIND, int D, int NT>
+int launch_tc(const PagedAttnLaunch& launch, cudaStream_t stream) {
+    using C = TcCfg<KIND, D, NT>;
+    constexpr int kSpace = 227 * 1024 - 2048 - 1024;  // less the static shared memory and the alignment
+    PagedAttnLaunch L = launch;
+    const int beside = C::BESIDE + (L.B + 1) * 4;
+    L.stages = (kSpace - beside) / (C::WARPS * C::TILE);
+    if (L.stages > C::STAGES) L.stages = C::STAGES;
+    const size_t smem = static_cast<size_t>(L.stages) * C::WARPS * C::TILE + beside + 1024;
+    if (cudaFuncSetAttribute(paged_tc_kernel<KIND, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem)) != cudaSuccess)
+        return ADA_ERR_LAUNCH;
+    paged_tc_kernel<KIND, D, NT><<<static_cast<unsigned>(L.n_cta), C::WARPS * 32, smem, stream>>>(L);
+    return cudaGetLastError() == cudaSuccess ? ADA_OK : ADA_ERR_LAUNCH;
+}
+
+template <int KIND>
+int launch_tc_kind(const PagedAttnLaunch& L, cudaStream_t stream) {
+    if (L.D == 64) return L.GB == 8 ? launch_tc<KIND, 64, 1>(L, stream) : launch_tc<KIND, 64, 2>(L, stream);
+    return L.GB == 8 ? launch_tc<KIND, 128, 1>(L, stream) : launch_tc<KIND, 128, 2>(L, stream);
+}
+
 }  // namespace
 
 int launch_paged_attn(const PagedAttnLaunch& L, cudaStream_t stream) {
     int rc;
     switch (L.kv_dtype) {
         case ADA_F32: rc = launch_simt_gb<ADA_F32>(L, stream); break;
-        case ADA_F16: rc = launch_simt_gb<ADA_F16>(L, stream); break;
-        case ADA_BF16: rc = launch_simt_gb<ADA_BF16>(L, stream); break;
-        case ADA_E4M3: rc = launch_simt_gb<ADA_E4M3>(L, stream); break;
+        case ADA_F16: rc = L.tc ? launch_tc_kind<1>(L, stream) : launch_simt_gb<ADA_F16>(L, stream); break;
+        case ADA_BF16: rc = L.tc ? launch_tc_kind<0>(L, stream) : launch_simt_gb<ADA_BF16>(L, stream); break;
+        case ADA_E4M3: rc = L.tc ? launch_tc_kind<2>(L, stream) : launch_simt_gb<ADA_E4M3>(L, stream); break;
         default: return ADA_ERR_DTYPE;
     }
-    if (rc) return rc;
+    if (rc || L.n_cta < 2) return rc;
     // The join starts while the last pieces run and waits for them on the device.
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(L.B) * L.U));
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3(static_cast<unsigned>(L.n_cta - 1), static_cast<unsigned>(L.GB < L.G ? L.GB : L.G));
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
