@@ -16,6 +16,7 @@ memory are left out and recorded in the library's status word
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -23,12 +24,23 @@ import torch
 from . import _lib
 from .config import ShapeError
 
+# Workspace sizes follow from the shapes alone; a decoding loop asks for the same ones again and again.
+@functools.lru_cache(maxsize=256)
+def _attn_workspace(b: int, h: int, hkv: int, d: int) -> int:
+    return max(_lib.load().ada_paged_attn_workspace_bytes(b, h, hkv, d), 1)
+
+
+@functools.lru_cache(maxsize=256)
+def _pages_workspace(num_pages: int, num_sequences: int, n: int) -> int:
+    return _lib.load().ada_pages_workspace_bytes(num_pages, num_sequences, n)
+
+
 Ids = Union[torch.Tensor, Sequence[int]]
 
 
 def _device_of(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> torch.device:
     dev = first.device
-    if dev.type != "cuda":
+    if not first.is_cuda:
         raise RuntimeError(f"adaattn_b200 runs on CUDA devices only (sm_100a); got a tensor on {dev}. "
                            "There is no CPU path.")
     for t in rest:
@@ -48,11 +60,12 @@ def _opt(t: Optional[torch.Tensor]):
 
 def _call(what: str, dev: torch.device, fn, *args) -> None:
     """One C call on the current stream of `dev`, with that device current."""
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, stream)
     if rc:
         _lib.check(rc, what)
 
@@ -104,8 +117,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                                                        torch.bfloat16):
         key_mask = key_mask.float()
     lib = _lib.load()
-    ws = torch.empty(max(lib.ada_paged_attn_workspace_bytes(b, h, max(1, k_pages.shape[1]), d), 1),
-                     dtype=torch.uint8, device=dev)
+    ws = torch.empty(_attn_workspace(b, h, max(1, k_pages.shape[1]), d), dtype=torch.uint8, device=dev)
     _call("ada_paged_attn", dev, lib.ada_paged_attn, _lib.tensor(_unit_last(q)), _lib.tensor(k_pages),
           _lib.tensor(v_pages), _lib.tensor(page_table), _lib.tensor(seq_lens), _opt(seqs), _opt(key_mask),
           _opt(k_scale), _opt(v_scale), float(d ** -0.5 if scale is None else scale), _lib.tensor(out),
@@ -138,18 +150,13 @@ def _planes(pages: torch.Tensor) -> _lib.AdaTensor:
     """[planes, P, ...] as [planes, P, elements of a page] (page blocks must be contiguous)."""
     if pages.dim() < 3:
         raise ShapeError(f"pages must be [planes, P, ...], got {pages.dim()}-D")
+    shape, stride = pages.shape, pages.stride()
     inner = 1
-    for n, s in zip(reversed(pages.shape[2:]), reversed(pages.stride()[2:])):
-        if n > 1 and s != inner:
+    for i in range(len(shape) - 1, 1, -1):
+        if shape[i] > 1 and stride[i] != inner:
             raise ShapeError("the pages' blocks must be contiguous")
-        inner *= n
-    t = _lib.AdaTensor()
-    t.data = pages.data_ptr() if pages.numel() else 0
-    t.dtype = _lib.tensor(pages[:0, :0].reshape(0)).dtype
-    t.ndim = 3
-    t.shape[0], t.shape[1], t.shape[2] = pages.shape[0], pages.shape[1], inner
-    t.stride[0], t.stride[1], t.stride[2] = pages.stride(0), pages.stride(1), 1
-    return t
+        inner *= shape[i]
+    return _lib.tensor(pages.as_strided((shape[0], shape[1], inner), (stride[0], stride[1], 1)))
 
 
 def _page_size(pages: torch.Tensor, page_size: Optional[int]) -> int:
@@ -163,8 +170,8 @@ def _page_size(pages: torch.Tensor, page_size: Optional[int]) -> int:
 def _workspace(page_table: torch.Tensor, ref_counts: torch.Tensor, n: int) -> torch.Tensor:
     if page_table.dim() != 2 or ref_counts.dim() != 1:
         raise ShapeError("page_table must be 2-D [S, W] and ref_counts 1-D [P]")
-    need = _lib.load().ada_pages_workspace_bytes(ref_counts.shape[0], page_table.shape[0], n)
-    return torch.empty(need, dtype=torch.uint8, device=page_table.device)
+    return torch.empty(_pages_workspace(ref_counts.shape[0], page_table.shape[0], n), dtype=torch.uint8,
+                       device=page_table.device)
 
 
 def reserve_pages(pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
