@@ -10,18 +10,27 @@
 //   dz_i = p_i (g_lse - g_lp - g_H (log p_i + H)) + g_lp [i = t].
 //
 // One pass over the logits: every thread keeps a running maximum, sum and
-// weighted sum (fp32, base 2), joined at the end, so HBM reads of V elements
-// bound it (each costs about six instructions, near half the issue rate at
-// full bandwidth). A row is shared by a cluster of CTAs when there are few
-// rows; its parts are joined through distributed shared memory, no workspace.
+// weighted sum (fp32, base 2, two of each in packed pairs), joined at the end.
+// A row is shared by a cluster of CTAs when there are few rows; its parts are
+// joined through distributed shared memory, no workspace.
+//
+// HBM reads of V elements bound it, if the instructions per element are few:
+// at 6.5 TB/s an SM takes 11.7 16-bit elements a cycle, of 128 instruction
+// lanes and 16 exponentials. Unpacking (1), clamping and the maximum on packed
+// pairs (1/2 each), argument, sum and weighted sum as packed fp32 pairs (1/2
+// each) and the exponential make 4.5. Logits are clamped from below (-2^100;
+// fp16: its lowest value) so that -inf stays out of the weighted sum; a row
+// with nothing above the clamp is done again by the plain formulas.
 //
 // Top k (k <= 64): candidates are 64-bit keys, the value's order above the
 // inverted column, so all keys differ and equal values rank by lowest index.
-// 128 thread pairs keep the maximum of what they saw; the k-th largest of
-// those bounds the k-th best logit from below, and only logits at or above
-// that bound enter the candidate list (a few k per row). The bound is renewed
-// at rounds 0, 1, 3, 7, ... The list is cut to its k best keys by radix
-// selection when it fills, whatever the order of the logits.
+// Every warp keeps its own list, so that no barrier is shared between them
+// while a row is read. 128 pairs of threads publish the largest logit they have
+// seen; the k-th largest of those, to 16 bits, bounds the k-th best logit from
+// below whenever it is read, and only logits at or above it enter a list (a
+// few k per row). It is found after the first round and renewed by one warp at
+// rounds 1, 3, 7, ... A list that fills, whatever the order of the logits, is
+// cut to its k best.
 #include <cooperative_groups.h>
 
 #include "ada_common.cuh"
@@ -33,12 +42,13 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kT = 256;             // threads
+constexpr int kWarps = kT / 32;
 constexpr int kPer = 16;            // elements per thread and round
 constexpr int kRound = kT * kPer;
-constexpr int kCap = 5120;          // candidates: kRound more than the cut's mark
-constexpr int kMark = kCap - kRound;
-constexpr int kGroups = kT / 2;
 constexpr int kMaxTop = 64;
+constexpr int kMark = 128;          // a warp's list is cut when it is longer after half a round
+constexpr int kList = kMark + 32 * kPer / 2;
+constexpr int kGroups = kT / 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -64,65 +74,73 @@ __device__ __forceinline__ int column_of(uint64_t key) {
 
 // ---- reading a row ---------------------------------------------------------------
 //
-// Columns are counted from the 16-byte boundary at or before the row's start,
+// Columns are counted from the 32-byte boundary at or before the row's start,
 // so vector loads are aligned whatever the row's address: column c = e - shift.
-// Vectors that reach past either end of the row are read element by element.
+// Vectors that reach past either end of the row are read element by element;
+// what is outside counts as -inf.
 template <int DT>
 struct Reader {
     static constexpr int EB = DT == ADA_F32 ? 4 : 2;
-    static constexpr int EPV = 16 / EB;         // elements per vector
+    static constexpr int EPV = 32 / EB;         // elements per vector
     static constexpr int NV = kPer / EPV;       // vectors per thread and round
+    static constexpr uint32_t kNegInf = DT == ADA_F32 ? 0xFF800000u : DT == ADA_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
     const uint8_t* base;  // the boundary
     int shift, V;
 
     __device__ Reader(const void* row, int v) : V(v) {
         const uint64_t a = reinterpret_cast<uint64_t>(row);
-        base = reinterpret_cast<const uint8_t*>(a & ~uint64_t(15));
-        shift = static_cast<int>(a & 15u) / EB;
+        base = reinterpret_cast<const uint8_t*>(a & ~uint64_t(31));
+        shift = static_cast<int>(a & 31u) / EB;
     }
     __device__ int rounds() const { return (V + shift + kRound - 1) / kRound; }
+    // Whether this thread's warp has columns in a round.
+    __device__ bool any(int round) const {
+        return round * kRound + static_cast<int>(threadIdx.x & ~31u) * EPV - shift < V;
+    }
     // First column of vector j of this thread in a round.
     __device__ int column(int round, int j) const {
         return ((round * NV + j) * kT + static_cast<int>(threadIdx.x)) * EPV - shift;
     }
-    __device__ void load(int round, uint4 (&w)[NV]) const {
+    __device__ void load(int round, uint32_t (&w)[NV * 8]) const {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = column(round, j);
             const uint8_t* p = base + static_cast<int64_t>(c + shift) * EB;
             if (c >= 0 && c + EPV <= V) {
-                w[j] = __ldcs(reinterpret_cast<const uint4*>(p));
-            } else {
-                uint32_t u[4];
+                asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                             : "=r"(w[8 * j]), "=r"(w[8 * j + 1]), "=r"(w[8 * j + 2]), "=r"(w[8 * j + 3]),
+                               "=r"(w[8 * j + 4]), "=r"(w[8 * j + 5]), "=r"(w[8 * j + 6]), "=r"(w[8 * j + 7])
+                             : "l"(p));
+            } else if (c >= V || c + EPV <= 0) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 8; ++i) w[8 * j + i] = kNegInf;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
                     if constexpr (DT == ADA_F32) {
-                        u[i] = (c + i >= 0 && c + i < V) ? reinterpret_cast<const uint32_t*>(p)[i] : 0xFF800000u;
+                        w[8 * j + i] = (c + i >= 0 && c + i < V) ? reinterpret_cast<const uint32_t*>(p)[i] : kNegInf;
                     } else {
-                        constexpr uint32_t kNegInf = DT == ADA_BF16 ? 0xFF80u : 0xFC00u;
                         const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-                        const uint32_t lo = (c + 2 * i >= 0 && c + 2 * i < V) ? h[2 * i] : kNegInf;
-                        const uint32_t hi = (c + 2 * i + 1 >= 0 && c + 2 * i + 1 < V) ? h[2 * i + 1] : kNegInf;
-                        u[i] = lo | (hi << 16);
+                        const uint32_t lo = (c + 2 * i >= 0 && c + 2 * i < V) ? h[2 * i] : kNegInf & 0xFFFFu;
+                        const uint32_t hi = (c + 2 * i + 1 >= 0 && c + 2 * i + 1 < V) ? h[2 * i + 1] : kNegInf & 0xFFFFu;
+                        w[8 * j + i] = lo | (hi << 16);
                     }
                 }
-                w[j] = make_uint4(u[0], u[1], u[2], u[3]);
             }
         }
     }
-    __device__ static void unpack(const uint4 (&w)[NV], float (&x)[kPer]) {
+    __device__ static void unpack(const uint32_t (&w)[NV * 8], float (&x)[kPer]) {
+        if constexpr (DT == ADA_F32) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+            for (int i = 0; i < kPer; ++i) x[i] = __uint_as_float(w[i]);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (DT == ADA_F32) {
-                    x[4 * j + i] = __uint_as_float(u[i]);
-                } else if constexpr (DT == ADA_BF16) {
-                    x[8 * j + 2 * i] = __uint_as_float(u[i] << 16);
-                    x[8 * j + 2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+            for (int i = 0; i < kPer / 2; ++i) {
+                if constexpr (DT == ADA_BF16) {
+                    x[2 * i] = __uint_as_float(w[i] << 16);
+                    x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
                 } else {
-                    unpack_f16x2(u[i], x[8 * j + 2 * i], x[8 * j + 2 * i + 1]);
+                    unpack_f16x2(w[i], x[2 * i], x[2 * i + 1]);
                 }
             }
         }
@@ -131,166 +149,349 @@ struct Reader {
 
 // ---- running sums ------------------------------------------------------------------
 
+// Packed pairs of 16-bit elements: maximum that keeps NaN.
+template <int DT>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (DT == ADA_BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ float lowest_kept() {
+    return DT == ADA_F16 ? -65504.f : -1.2676506e30f;  // fp16's lowest value, -2^100
+}
+// A row maximum at which the clamp or m log2 e does not hold (NaN too).
+template <int DT>
+__device__ __forceinline__ bool ends_of_range(float m) {
+    return !(fabsf(m) <= -lowest_kept<DT>()) || m == lowest_kept<DT>();
+}
+template <int DT>
+__device__ __forceinline__ void unpack_pair(uint32_t w, float& lo, float& hi) {
+    if constexpr (DT == ADA_BF16) {
+        lo = __uint_as_float(w << 16);
+        hi = __uint_as_float(w & 0xFFFF0000u);
+    } else {
+        unpack_f16x2(w, lo, hi);
+    }
+}
+
+// With x_i = z_i log2 e and M = m log2 e rounded: s = sum 2^(x_i - M), t = sum (x_i - M) 2^(x_i - M).
 struct Sums {
-    float m, s, t;  // maximum; sum of 2^x and of x 2^x with x = (z - m) log2 e
+    float m, s, t;
 };
 
-// Changes the maximum to m (at least s.m).
-__device__ __forceinline__ void shift_to(Sums& a, float m) {
-    if (a.s != 0.f) {
-        const float d = (a.m - m) * kLog2e;
-        const float w = exp2f(d);
-        a.t = w == 0.f ? 0.f : w * fmaf(a.s, d, a.t);
-        a.s *= w;
+// What a change of the maximum from a to b adds to the exponents.
+__device__ __forceinline__ float exponent_shift(float a, float b) { return a * kLog2e - b * kLog2e; }
+
+__device__ __forceinline__ void shift_sums(float d, float& s, float& t) {
+    if (s == 0.f) return;
+    const float w = exp2f(d);
+    t = w == 0.f ? 0.f : w * fmaf(s, d, t);
+    s *= w;
+}
+// The sums of the first n lanes of a warp (n a power of two), in every one of them.
+__device__ __forceinline__ Sums join_warp(Sums a, int n) {
+    float m = a.m;
+    for (int o = n / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    shift_sums(exponent_shift(a.m, m), a.s, a.t);
+    for (int o = n / 2; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
     }
     a.m = m;
-}
-__device__ __forceinline__ Sums join(Sums a, Sums b) {
-    const float m = max_nan(a.m, b.m);
-    shift_to(a, m);
-    shift_to(b, m);
-    return Sums{m, a.s + b.s, a.t + b.t};
+    return a;
 }
 
-__device__ __forceinline__ void add_elements(Sums& a, const float (&x)[kPer], float top) {
-    if (!(top <= a.m)) shift_to(a, top);  // NaN too
-    const float ref = a.m == -INFINITY ? 0.f : a.m;
+// A thread's sums in two halves.
+struct PairSums {
+    float m;
+    uint64_t s, t;
+};
+
+// One round's elements; returns their maximum (clamped).
+template <int DT>
+__device__ __forceinline__ float add_round(PairSums& a, const uint32_t (&w)[Reader<DT>::NV * 8]) {
+    uint32_t v[Reader<DT>::NV * 8];
+    float top;
+    if constexpr (DT == ADA_F32) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        // -inf (and what is as far below) counts as -1e30: its power is 0 and so is the product
-        const float d = max_nan((x[i] - ref) * kLog2e, -1e30f);
-        const float e = fast_exp2(d);
-        a.s += e;
-        a.t = fmaf(e, d, a.t);
+        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(max_nan(__uint_as_float(w[i]), lowest_kept<DT>()));
+        float q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            q[i] = max_nan(max_nan(__uint_as_float(v[i]), __uint_as_float(v[i + 4])),
+                           max_nan(__uint_as_float(v[i + 8]), __uint_as_float(v[i + 12])));
+        top = max_nan(max_nan(q[0], q[1]), max_nan(q[2], q[3]));
+    } else {
+        constexpr uint32_t kClamp = DT == ADA_BF16 ? 0xF180F180u : 0xFBFFFBFFu;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = max2_nan<DT>(w[i], kClamp);
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = max2_nan<DT>(v[i], v[i + 4]);
+        q[0] = max2_nan<DT>(max2_nan<DT>(q[0], q[1]), max2_nan<DT>(q[2], q[3]));
+        float lo, hi;
+        unpack_pair<DT>(q[0], lo, hi);
+        top = max_nan(lo, hi);
     }
+    if (!(top <= a.m)) {  // NaN too
+        const float d = exponent_shift(a.m, top);
+        float s0, s1, t0, t1;
+        f2_unpack(a.s, s0, s1);
+        f2_unpack(a.t, t0, t1);
+        shift_sums(d, s0, t0);
+        shift_sums(d, s1, t1);
+        a.s = f2_pack(s0, s1);
+        a.t = f2_pack(t0, t1);
+        a.m = top;
+    }
+    const uint64_t l2 = f2_splat(kLog2e), m2 = f2_splat(-(a.m * kLog2e));
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) {
+        uint64_t x;
+        if constexpr (DT == ADA_F32) {
+            x = f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        } else {
+            float lo, hi;
+            unpack_pair<DT>(v[i], lo, hi);
+            x = f2_pack(lo, hi);
+        }
+        const uint64_t d = f2_fma(x, l2, m2);
+        float d0, d1;
+        f2_unpack(d, d0, d1);
+        const uint64_t e = f2_pack(fast_exp2(d0), fast_exp2(d1));
+        a.s = f2_add(a.s, e);
+        a.t = f2_fma(e, d, a.t);
+    }
+    return top;
+}
+
+// A row without a logit above the clamp, by the whole block: m, and s and t of x_i - m itself.
+template <int DT>
+__device__ Sums plain_sums(const Reader<DT>& R, Sums* s_warp) {
+    Sums a{-INFINITY, 0.f, 0.f};
+    for (int pass = 0; pass < 2; ++pass) {
+        const float ref = a.m == -INFINITY ? 0.f : a.m;
+        for (int r = 0; r < R.rounds(); ++r) {
+            uint32_t w[Reader<DT>::NV * 8];
+            float x[kPer];
+            R.load(r, w);
+            Reader<DT>::unpack(w, x);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (pass == 0) {
+                    a.m = max_nan(a.m, x[i]);
+                } else {
+                    const float d = max_nan((x[i] - ref) * kLog2e, -1e30f);
+                    const float e = exp2f(d);
+                    a.s += e;
+                    a.t = fmaf(e, d, a.t);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            a.m = max_nan(a.m, __shfl_xor_sync(0xffffffffu, a.m, o));
+            a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+            a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+        }
+        if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = a;
+        __syncthreads();
+        for (int i = 0; i < kWarps; ++i) a.m = max_nan(a.m, s_warp[i].m);
+    }
+    a.s = a.t = 0.f;
+    for (int i = 0; i < kWarps; ++i) {
+        a.s += s_warp[i].s;
+        a.t += s_warp[i].t;
+    }
+    return a;
 }
 
 // ---- top k ---------------------------------------------------------------------------
 
 struct TopState {
-    uint64_t cand[kCap];
-    uint64_t best[kMaxTop];
-    uint64_t group[kGroups];
-    uint64_t bound;   // candidates are keys above it
-    int count, n_best;
+    uint64_t list[kWarps][kList];
+    uint64_t best[8 * kMaxTop];    // the row's best, then those of the cluster's other parts
+    uint64_t sorted[kMaxTop];
+    float seen[kGroups];           // largest logit of a pair of threads so far
+    uint32_t bound;                // the highest bound found so far, as an order (0: none)
+    int count[kWarps];
+    int n_best;
     uint32_t hist[256];
     uint32_t digit, below;
 };
 
-// The k best of the first n candidates to best[] (unordered); n > k. Radix
-// selection of the k-th largest key, a byte at a time; all keys differ.
-__device__ void cut(TopState& S, int n, int k) {
-    uint64_t prefix = 0, mask = 0;
-    int want = k;
-    for (int b = 56; b >= 0; b -= 8) {
-        S.hist[threadIdx.x] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kT)
-            if ((S.cand[i] & mask) == prefix) atomicAdd(&S.hist[(S.cand[i] >> b) & 255u], 1u);
-        __syncthreads();
-        if (threadIdx.x < 32) {  // lane l: digits 255 - 8 l downwards
-            uint32_t c[8], sum = 0;
+// Order of a value as an unsigned number (NaN above all).
+__device__ __forceinline__ uint32_t order_of(float x) { return static_cast<uint32_t>(key_of(x, 0) >> 32); }
+
+// The k-th largest of what groups of threads have seen, as an order rounded
+// down to its first 16 bits; 0 where that is not above the clamp. By one warp,
+// without a barrier: a value read too early is smaller and its bound holds all
+// the same. G groups per lane (32 G in all): more for larger k, as the k-th
+// largest of n groups' maxima has about n log(n / (n - k)) logits above it.
+template <int DT, int G>
+__device__ __forceinline__ uint32_t find_bound_of(const TopState& S, int k) {
+    const int lane = threadIdx.x & 31;
+    uint32_t v[G];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                c[i] = S.hist[255 - 8 * threadIdx.x - i];
-                sum += c[i];
-            }
-            uint32_t scan = sum;
+    for (int i = 0; i < G; ++i) {
+        float x = -INFINITY;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t up = __shfl_up_sync(0xffffffffu, scan, o);
-                if (threadIdx.x >= o) scan += up;
-            }
-            uint32_t before = scan - sum;
-            if (before < want && scan >= want) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (before < want && before + c[i] >= want) {
-                        S.digit = 255 - 8 * threadIdx.x - i;
-                        S.below = before;
-                        break;
-                    }
-                    before += c[i];
-                }
-            }
-        }
-        __syncthreads();
-        prefix |= static_cast<uint64_t>(S.digit) << b;
-        mask |= uint64_t(255) << b;
-        want -= static_cast<int>(S.below);
+        for (int j = 0; j < 4 / G; ++j)
+            x = max_nan(x, *const_cast<const volatile float*>(&S.seen[(i * (4 / G) + j) * 32 + lane]));
+        v[i] = order_of(x);
     }
+    uint32_t prefix = 0;
+#pragma unroll 1
+    for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+        const uint32_t c = prefix | bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < G; ++i) n += __popc(__ballot_sync(0xffffffffu, v[i] >= c));
+        if (n >= k) prefix = c;
+    }
+    return prefix <= order_of(lowest_kept<DT>()) ? 0u : prefix;
+}
+template <int DT>
+__device__ uint32_t find_bound(const TopState& S, int k) {
+    return k <= 8 ? find_bound_of<DT, 1>(S, k) : k <= 24 ? find_bound_of<DT, 2>(S, k) : find_bound_of<DT, 4>(S, k);
+}
+
+// Cuts a warp's list of n > k keys to its k best and returns the smallest of
+// them: the k-th largest key, bit by bit.
+__device__ uint64_t cut_list(uint64_t* list, int n, int k) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    uint64_t prefix = 0;
+#pragma unroll 1
+    for (int b = 63; b >= 0; --b) {
+        const uint64_t c = prefix | (uint64_t(1) << b);
+        int have = 0;
+        for (int i = lane; i - lane < n; i += 32) have += __popc(__ballot_sync(0xffffffffu, i < n && list[i] >= c));
+        if (have >= k) prefix = c;
+    }
+    int kept = 0;
+    for (int i = lane; i - lane < n; i += 32) {  // kept <= i: nothing unread is overwritten
+        const uint64_t key = i < n ? list[i] : 0;
+        const bool take = i < n && key >= prefix;
+        const uint32_t who = __ballot_sync(0xffffffffu, take);
+        if (take) list[kept + __popc(who & ((1u << lane) - 1u))] = key;
+        kept += __popc(who);
+        __syncwarp();
+    }
+    return prefix;
+}
+
+// The k best keys of the first n of best[] (n <= 512), in order, to sorted[].
+__device__ void sort_best(TopState& S, int n, int k) {
+    for (int i = threadIdx.x; i < n; i += kT) {
+        const uint64_t mine = S.best[i];
+        int r = 0;
+        for (int j = 0; j < n; ++j) r += S.best[j] > mine;
+        if (r < k) S.sorted[r] = mine;
+    }
+    __syncthreads();
+}
+
+// The block's k best keys (all it has, when fewer), in order, to sorted[].
+template <int DT>
+__device__ void gather_best(TopState& S, int k) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) S.n_best = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kT)
-        if (S.cand[i] >= prefix) S.best[atomicAdd(&S.n_best, 1)] = S.cand[i];
+    uint64_t from = static_cast<uint64_t>(S.bound) << 32;
+    const int len = S.count[warp];
+    int mine = 0;
+    for (int i = lane; i < len; i += 32) mine += S.list[warp][i] >= from;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) atomicAdd(&S.n_best, mine);
     __syncthreads();
-    if (threadIdx.x == 0 && prefix > S.bound + 1) S.bound = prefix - 1;
+    const int n = S.n_best;
+    __syncthreads();
+    if (threadIdx.x == 0) S.n_best = 0;
+    if (n > 8 * kMaxTop) {  // many equal logits: the exact k-th largest key, a byte at a time
+        uint64_t prefix = 0, mask = 0;
+        int want = k;
+        for (int b = 56; b >= 0; b -= 8) {
+            S.hist[threadIdx.x] = 0;
+            __syncthreads();
+            for (int i = lane; i < len; i += 32) {
+                const uint64_t key = S.list[warp][i];
+                if ((key & mask) == prefix) atomicAdd(&S.hist[(key >> b) & 255u], 1u);
+            }
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                int d = 255, before = 0;
+                while (d > 0 && before + static_cast<int>(S.hist[d]) < want) before += static_cast<int>(S.hist[d--]);
+                S.digit = static_cast<uint32_t>(d);
+                S.below = static_cast<uint32_t>(before);
+            }
+            __syncthreads();
+            prefix |= static_cast<uint64_t>(S.digit) << b;
+            mask |= uint64_t(255) << b;
+            want -= static_cast<int>(S.below);
+        }
+        from = prefix;
+    }
+    __syncthreads();
+    for (int i = lane; i < len; i += 32) {
+        const uint64_t key = S.list[warp][i];
+        if (key >= from) S.best[atomicAdd(&S.n_best, 1)] = key;
+    }
+    __syncthreads();
+    sort_best(S, S.n_best, k);
+    if (threadIdx.x == 0) S.n_best = min(S.n_best, k);
+    __syncthreads();
 }
 
-// The k best candidates, in order, to best[0 .. n_best).
-__device__ void rank_best(TopState& S, int k) {
-    int n = S.count;
-    if (n > 512) {
-        cut(S, n, k);
-        n = k;
-        for (int i = threadIdx.x; i < n; i += kT) S.cand[i] = S.best[i];
-        __syncthreads();
-    }
-    for (int i = threadIdx.x; i < n; i += kT) {
-        const uint64_t mine = S.cand[i];
-        int r = 0;
-        for (int j = 0; j < n; ++j) r += S.cand[j] > mine;
-        if (r < k) S.best[r] = mine;
-    }
-    if (threadIdx.x == 0) S.n_best = min(n, k);
-    __syncthreads();
-}
-
-// One round of logits. `seen`: the largest logit this thread has met.
+// One round's elements for the lists. `seen`: the largest logit this thread
+// has met; `exact`: keys below it are out of this warp's k best.
 template <int DT>
-__device__ __forceinline__ void top_round(TopState& S, int k, const float (&x)[kPer], float top, float& seen, int turn,
-                                          const Reader<DT>& R, int round) {
+__device__ __forceinline__ void top_round(TopState& S, int k, const uint32_t (&w)[Reader<DT>::NV * 8], float top, float& seen,
+                                          uint64_t& exact, int turn, const Reader<DT>& R, int round) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     seen = max_nan(seen, top);
     if ((turn & (turn + 1)) == 0) {  // 0, 1, 3, 7, ...
-        const float other = __shfl_xor_sync(0xffffffffu, seen, 1);
-        // one key per pair: the value alone decides, pairs of one value count by their number
-        const uint64_t g = key_of(max_nan(seen, other), threadIdx.x >> 1);
-        if ((threadIdx.x & 1) == 0) S.group[threadIdx.x >> 1] = g;
-        __syncthreads();
-        if (threadIdx.x < kGroups) {
-            const uint64_t mine = S.group[threadIdx.x];
-            int r = 0;
-#pragma unroll 8
-            for (int j = 0; j < kGroups; ++j) r += S.group[j] > mine;
-            if (r == k - 1) {
-                const uint64_t bound = (mine >> 32) << 32;  // every column of that value passes
-                if (bound != 0 && bound - 1 > S.bound && value_of(mine) != -INFINITY) S.bound = bound - 1;
-            }
+        const float pair = max_nan(seen, __shfl_xor_sync(0xffffffffu, seen, 1));
+        if ((lane & 1) == 0) *const_cast<volatile float*>(&S.seen[threadIdx.x >> 1]) = pair;
+        if (turn == 0) __syncthreads();
+        __syncwarp();
+        if (warp == (turn & (kWarps - 1))) {
+            const uint32_t b = find_bound<DT>(S, k);
+            if (lane == 0) atomicMax(&S.bound, b);
+            __syncwarp();
         }
-        __syncthreads();
+        if (turn == 0) __syncthreads();
     }
-    const uint64_t bound = S.bound;
-    const uint32_t hi = static_cast<uint32_t>((bound + 1) >> 32);
-    const float low = hi == 0 ? -INFINITY : value_of(static_cast<uint64_t>(hi) << 32);
-    if (!(top < low)) {
+    if (!R.any(round)) return;
+    const uint32_t bound = *const_cast<const volatile uint32_t*>(&S.bound);
+    const float low = bound == 0u ? -INFINITY : value_of(static_cast<uint64_t>(bound) << 32);
+    if (__any_sync(0xffffffffu, !(top < low))) {
+        float x[kPer];
+        Reader<DT>::unpack(w, x);
+        int n = S.count[warp];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             constexpr int EPV = Reader<DT>::EPV;
-            if (x[i] < low) continue;
             const int c = R.column(round, i / EPV) + i % EPV;
-            if (c < 0 || c >= R.V) continue;
-            const uint64_t key = key_of(x[i], c);
-            if (key > bound) S.cand[atomicAdd(&S.count, 1)] = key;
+            if (__any_sync(0xffffffffu, !(x[i] < low))) {
+                const uint64_t key = key_of(x[i], c);
+                const bool take = (key >> 32) >= bound && key >= exact && c >= 0 && c < R.V;
+                const uint32_t who = __ballot_sync(0xffffffffu, take);
+                if (take) S.list[warp][n + __popc(who & ((1u << lane) - 1u))] = key;
+                n += __popc(who);
+            }
+            if ((i + 1) % (kPer / 2) == 0 && n > kMark) {
+                exact = cut_list(S.list[warp], n, k);
+                n = k;
+            }
         }
-    }
-    __syncthreads();
-    const int n = S.count;
-    __syncthreads();
-    if (n > kMark) {
-        cut(S, n, k);
-        for (int i = threadIdx.x; i < k; i += kT) S.cand[i] = S.best[i];
-        if (threadIdx.x == 0) S.count = k;
-        __syncthreads();
+        __syncwarp();
+        if (lane == 0) S.count[warp] = n;
+        __syncwarp();
     }
 }
 
@@ -299,7 +500,7 @@ __device__ __forceinline__ void top_round(TopState& S, int k, const float (&x)[k
 template <int DT, bool TOP>
 __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constant__ LogprobLaunch L) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ Sums s_warp[kT / 32];
+    __shared__ Sums s_warp[kWarps];
     __shared__ Sums s_part;
     TopState& S = *reinterpret_cast<TopState*>(smem);
     cg::cluster_group cluster = cg::this_cluster();
@@ -310,62 +511,60 @@ __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constan
     const uint8_t* zr = static_cast<const uint8_t*>(L.logits) + off * EB;
     const Reader<DT> R(zr, L.V);
     const int k = TOP ? L.top : 0;
-    if (TOP && threadIdx.x == 0) {
-        S.bound = 0;
-        S.count = 0;
-        S.n_best = 0;
+    if constexpr (TOP) {
+        if (threadIdx.x < kGroups) S.seen[threadIdx.x] = -INFINITY;
+        if (threadIdx.x < kWarps) S.count[threadIdx.x] = 0;
+        if (threadIdx.x == 0) S.bound = 0;
+        __syncthreads();
     }
-    if (TOP) __syncthreads();
-    Sums a{-INFINITY, 0.f, 0.f};
+    PairSums sums{-INFINITY, f2_splat(0.f), f2_splat(0.f)};
     float seen = -INFINITY;
+    uint64_t exact = 0;
     const int rounds = R.rounds();
-    uint4 w[Reader<DT>::NV];
+    uint32_t w[Reader<DT>::NV * 8], next[Reader<DT>::NV * 8];
     if (rank < rounds) R.load(rank, w);
     int turn = 0;
     for (int r = rank; r < rounds; r += parts, ++turn) {
-        float x[kPer];
-        Reader<DT>::unpack(w, x);
-        if (r + parts < rounds) R.load(r + parts, w);
-        float top = x[0];
+        if (r + parts < rounds) R.load(r + parts, next);
+        float top = -INFINITY;
+        if (R.any(r)) top = add_round<DT>(sums, w);
+        if constexpr (TOP) top_round<DT>(S, k, w, top, seen, exact, turn, R, r);
 #pragma unroll
-        for (int i = 1; i < kPer; ++i) top = max_nan(top, x[i]);
-        add_elements(a, x, top);
-        if constexpr (TOP) top_round<DT>(S, k, x, top, seen, turn, R, r);
+        for (int j = 0; j < Reader<DT>::NV * 8; ++j) w[j] = next[j];
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Sums b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
-        a = join(a, b);
+    Sums a;
+    {
+        float s0, s1, t0, t1;
+        f2_unpack(sums.s, s0, s1);
+        f2_unpack(sums.t, t0, t1);
+        a = join_warp(Sums{sums.m, s0 + s1, t0 + t1}, 32);
     }
     if ((threadIdx.x & 31) == 0) s_warp[threadIdx.x >> 5] = a;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < kT / 32; ++i) a = join(a, s_warp[i]);
-        s_part = a;
+    if (threadIdx.x < 32) {
+        a = join_warp(threadIdx.x < kWarps ? s_warp[threadIdx.x] : Sums{-INFINITY, 0.f, 0.f}, kWarps);
+        if (threadIdx.x == 0) s_part = a;
     }
-    if (TOP) rank_best(S, k);
+    if constexpr (TOP) gather_best<DT>(S, k);
     if (parts > 1) {
         cluster.sync();
         if (rank == 0) {
-            if (threadIdx.x == 0) {
-                for (int i = 1; i < parts; ++i) a = join(a, *cluster.map_shared_rank(&s_part, i));
-                s_part = a;
+            if (threadIdx.x < 32) {
+                a = join_warp(threadIdx.x < parts ? *cluster.map_shared_rank(&s_part, threadIdx.x)
+                                                  : Sums{-INFINITY, 0.f, 0.f}, 8);
+                __syncwarp();
+                if (threadIdx.x == 0) s_part = a;
             }
-            if (TOP) {
+            if constexpr (TOP) {
                 int n = 0;
                 for (int i = 0; i < parts; ++i) {
                     const TopState* T = cluster.map_shared_rank(&S, i);
                     const int m = T->n_best;
-                    for (int j = threadIdx.x; j < m; j += kT) S.cand[n + j] = T->best[j];
+                    for (int j = threadIdx.x; j < m; j += kT) S.best[n + j] = T->sorted[j];
                     n += m;
                 }
                 __syncthreads();
-                if (threadIdx.x == 0) S.count = n;
-                __syncthreads();
-                rank_best(S, k);
+                sort_best(S, n, k);
             }
         }
         cluster.sync();  // the parts stay until they are read
@@ -373,7 +572,18 @@ __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constan
     }
     __syncthreads();
     a = s_part;
-    const float ls = logf(a.s);
+    if (!ends_of_range<DT>(a.m) && threadIdx.x >= (TOP ? kMaxTop : 32)) return;
+    // ls = log sum exp(z_i - m), mean = sum p_i (z_i - m), in base 2 first
+    float ls, mean;
+    if (ends_of_range<DT>(a.m)) {
+        a = plain_sums<DT>(R, s_warp);
+        ls = logf(a.s);
+        mean = a.t / a.s * kLn2;
+    } else {
+        const float r = fmaf(a.m, kLog2e, -(a.m * kLog2e));  // what M's rounding left out
+        ls = (log2f(a.s) - r) * kLn2;
+        mean = (a.t / a.s - r) * kLn2;
+    }
     if (threadIdx.x == 0) {
         const int64_t t = L.tok64 ? static_cast<const int64_t*>(L.tokens)[row] : static_cast<const int32_t*>(L.tokens)[row];
         float lp = 0.f;
@@ -386,14 +596,14 @@ __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constan
             }
         }
         L.logprobs[row] = lp;
-        L.entropy[row] = ls - a.t / a.s * kLn2;
+        L.entropy[row] = ls - mean;
         L.lse[row] = a.m + ls;
         L.stats[2 * row] = a.m;
         L.stats[2 * row + 1] = ls;
     }
     if constexpr (TOP) {
         for (int i = threadIdx.x; i < k; i += kT) {
-            const int c = column_of(S.best[i]);
+            const int c = column_of(S.sorted[i]);
             L.top_tokens[row * k + i] = c;
             L.top_logprobs[row * k + i] = (load_as_f32(zr, c, DT) - a.m) - ls;
         }
@@ -411,7 +621,7 @@ __global__ void __launch_bounds__(kT) token_logprobs_bwd_kernel(const __grid_con
     const int64_t a = row / L.R, b = row % L.R;
     const Reader<DT> R(static_cast<const uint8_t*>(L.logits) + (a * L.s0 + b * L.s1) * EB, L.V);
     uint8_t* gr = static_cast<uint8_t*>(L.grad) + (a * L.gs0 + b * L.gs1) * EB;
-    const bool aligned = (reinterpret_cast<uint64_t>(gr) & 15u) / EB == static_cast<uint64_t>(R.shift);
+    const bool aligned = (reinterpret_cast<uint64_t>(gr) & 31u) / EB == static_cast<uint64_t>(R.shift);
     const float m = L.stats[2 * row], ls = L.stats[2 * row + 1];
     const int64_t t = L.tok64 ? static_cast<const int64_t*>(L.tokens)[row] : static_cast<const int32_t*>(L.tokens)[row];
     float g_lp = (L.g_logprobs != nullptr && t != L.ignore) ? L.g_logprobs[row] : 0.f;
@@ -420,8 +630,15 @@ __global__ void __launch_bounds__(kT) token_logprobs_bwd_kernel(const __grid_con
     const float g_lse = L.g_lse != nullptr ? L.g_lse[row] : 0.f;
     const float c0 = g_lse - g_lp - g_h * L.entropy[row];
     const int rounds = R.rounds();
+    // log2 p = (x - M) + shift with M as the forward's; rows near the ends of the range take the plain difference
+    const bool plain = ends_of_range<DT>(m);
+    const float M = plain ? 0.f : m * kLog2e;
+    const float shift = plain ? 0.f : -fmaf(ls, kLog2e, fmaf(m, kLog2e, -M));
+    const uint64_t l2 = f2_splat(kLog2e), m2 = f2_splat(-M), sh2 = f2_splat(shift);
+    const uint64_t c2 = f2_splat(c0), gh2 = f2_splat(-g_h * kLn2);
     for (int r = seg; r < rounds; r += L.segments) {
-        uint4 w[NV];
+        if (!R.any(r)) break;
+        uint32_t w[NV * 8];
         float x[kPer];
         R.load(r, w);
         Reader<DT>::unpack(w, x);
@@ -430,21 +647,34 @@ __global__ void __launch_bounds__(kT) token_logprobs_bwd_kernel(const __grid_con
             const int c = R.column(r, j);
             float g[EPV];
 #pragma unroll
-            for (int i = 0; i < EPV; ++i) {
-                const float logp = (x[j * EPV + i] - m) - ls;
-                const float p = exp2f(logp * kLog2e);
-                g[i] = p == 0.f ? 0.f * c0 : p * fmaf(-g_h, logp, c0);
-                if (c + i == t) g[i] += g_lp;
+            for (int i = 0; i < EPV; i += 2) {
+                float d0, d1;
+                if (plain) {
+                    d0 = ((x[j * EPV + i] - m) - ls) * kLog2e;
+                    d1 = ((x[j * EPV + i + 1] - m) - ls) * kLog2e;
+                } else {
+                    f2_unpack(f2_add(f2_fma(f2_pack(x[j * EPV + i], x[j * EPV + i + 1]), l2, m2), sh2), d0, d1);
+                }
+                // p is 0 from -150 on: the bound keeps -inf out of the product
+                d0 = max_nan(d0, -1000.f);
+                d1 = max_nan(d1, -1000.f);
+                const uint64_t e = f2_pack(fast_exp2(d0), fast_exp2(d1));
+                f2_unpack(f2_mul(e, f2_fma(gh2, f2_pack(d0, d1), c2)), g[i], g[i + 1]);
             }
-            uint32_t u[4];
+            if (t >= c && t < c + EPV) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < EPV; ++i)
+                    if (c + i == t) g[i] += g_lp;
+            }
+            uint32_t u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
                 if constexpr (DT == ADA_F32) u[i] = __float_as_uint(g[i]);
                 else if constexpr (DT == ADA_BF16) u[i] = pack_bf16x2(g[2 * i], g[2 * i + 1]);
                 else u[i] = pack_f16x2(g[2 * i], g[2 * i + 1]);
             }
             if (aligned && c >= 0 && c + EPV <= L.V) {
-                __stcs(reinterpret_cast<uint4*>(gr + static_cast<int64_t>(c) * EB), make_uint4(u[0], u[1], u[2], u[3]));
+                st_global_v8(gr + static_cast<int64_t>(c) * EB, u);
             } else {
 #pragma unroll
                 for (int i = 0; i < EPV; ++i) {

@@ -42,11 +42,11 @@ def _rows3(t: torch.Tensor) -> torch.Tensor:
 
 
 def _grad_like(z3: torch.Tensor) -> torch.Tensor:
-    """An empty tensor of z3's shape whose rows start like z3's relative to 16
+    """An empty tensor of z3's shape whose rows start like z3's relative to 32
     bytes, so that both are read and written in the same vectors. Rows of
     vocabulary-sized views (a padded matrix) stay padded in memory."""
     a, r, v = z3.shape
-    unit = 16 // z3.element_size()
+    unit = 32 // z3.element_size()
     ld = z3.stride(1) if r > 1 else z3.stride(0) if a > 1 else v
     if ld < v or ld > v + 1024 or (a > 1 and r > 1 and z3.stride(0) % unit != (r * ld) % unit):
         ld = (v + unit - 1) // unit * unit
