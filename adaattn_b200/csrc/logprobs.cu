@@ -24,13 +24,14 @@
 //
 // Top k (k <= 64): candidates are 64-bit keys, the value's order above the
 // inverted column, so all keys differ and equal values rank by lowest index.
-// Every warp keeps its own list, so that no barrier is shared between them
-// while a row is read. 128 pairs of threads publish the largest logit they have
-// seen; the k-th largest of those, to 16 bits, bounds the k-th best logit from
-// below whenever it is read, and only logits at or above it enter a list (a
-// few k per row). It is found after the first round and renewed by one warp at
-// rounds 1, 3, 7, ... A list that fills, whatever the order of the logits, is
-// cut to its k best.
+// While the row is read, a thread only keeps the largest logit it has seen,
+// the vector that held it, and the second largest of its vectors' maxima. The
+// k-th largest of 128 thread pairs' maxima bounds the k-th best logit from
+// below, and what reaches it lies with the few threads (about k) whose maximum
+// does: each reads that one vector again (L2), and the rare thread whose second
+// vector reaches the bound too has all its vectors read by its warp. The logits
+// at or above the bound are sorted. A row with more of them than fit (masked or
+// constant rows) takes radix passes over all its keys instead.
 #include <cooperative_groups.h>
 
 #include "ada_common.cuh"
@@ -46,8 +47,7 @@ constexpr int kWarps = kT / 32;
 constexpr int kPer = 16;            // elements per thread and round
 constexpr int kRound = kT * kPer;
 constexpr int kMaxTop = 64;
-constexpr int kMark = 128;          // a warp's list is cut when it is longer after half a round
-constexpr int kList = kMark + 32 * kPer / 2;
+constexpr int kCand = 2304;         // candidates: 32 k of a sorted row and some
 constexpr int kGroups = kT / 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -63,10 +63,6 @@ __device__ __forceinline__ uint64_t key_of(float x, int col) {
     const uint32_t b = __float_as_uint(x + 0.f);  // -0 ranks as 0
     const uint32_t o = isnan(x) ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
     return (static_cast<uint64_t>(o) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(col));
-}
-__device__ __forceinline__ float value_of(uint64_t key) {
-    const uint32_t o = static_cast<uint32_t>(key >> 32);
-    return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
 __device__ __forceinline__ int column_of(uint64_t key) {
     return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key));
@@ -84,13 +80,15 @@ struct Reader {
     static constexpr int EPV = 32 / EB;         // elements per vector
     static constexpr int NV = kPer / EPV;       // vectors per thread and round
     static constexpr uint32_t kNegInf = DT == ADA_F32 ? 0xFF800000u : DT == ADA_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
-    const uint8_t* base;  // the boundary
-    int shift, V;
+    const uint8_t* mine;  // this thread's first vector
+    int c0, V;            // its column
+    int shift;
 
     __device__ Reader(const void* row, int v) : V(v) {
         const uint64_t a = reinterpret_cast<uint64_t>(row);
-        base = reinterpret_cast<const uint8_t*>(a & ~uint64_t(31));
         shift = static_cast<int>(a & 31u) / EB;
+        mine = reinterpret_cast<const uint8_t*>(a & ~uint64_t(31)) + threadIdx.x * 32;
+        c0 = static_cast<int>(threadIdx.x) * EPV - shift;
     }
     __device__ int rounds() const { return (V + shift + kRound - 1) / kRound; }
     // Whether this thread's warp has columns in a round.
@@ -98,44 +96,43 @@ struct Reader {
         return round * kRound + static_cast<int>(threadIdx.x & ~31u) * EPV - shift < V;
     }
     // First column of vector j of this thread in a round.
-    __device__ int column(int round, int j) const {
-        return ((round * NV + j) * kT + static_cast<int>(threadIdx.x)) * EPV - shift;
-    }
-    __device__ void load(int round, uint32_t (&w)[NV * 8]) const {
+    __device__ int column(int round, int j) const { return round * kRound + j * kT * EPV + c0; }
+    // The vector that begins at column c.
+    __device__ void vector(int c, uint32_t* w) const {
+        const uint8_t* p = mine + static_cast<int64_t>(c - c0) * EB;
+        if (c >= 0 && c <= V - EPV) {
+            asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(p));
+        } else if (c >= V || c + EPV <= 0) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = column(round, j);
-            const uint8_t* p = base + static_cast<int64_t>(c + shift) * EB;
-            if (c >= 0 && c + EPV <= V) {
-                asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                             : "=r"(w[8 * j]), "=r"(w[8 * j + 1]), "=r"(w[8 * j + 2]), "=r"(w[8 * j + 3]),
-                               "=r"(w[8 * j + 4]), "=r"(w[8 * j + 5]), "=r"(w[8 * j + 6]), "=r"(w[8 * j + 7])
-                             : "l"(p));
-            } else if (c >= V || c + EPV <= 0) {
+            for (int i = 0; i < 8; ++i) w[i] = kNegInf;
+        } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[8 * j + i] = kNegInf;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if constexpr (DT == ADA_F32) {
-                        w[8 * j + i] = (c + i >= 0 && c + i < V) ? reinterpret_cast<const uint32_t*>(p)[i] : kNegInf;
-                    } else {
-                        const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-                        const uint32_t lo = (c + 2 * i >= 0 && c + 2 * i < V) ? h[2 * i] : kNegInf & 0xFFFFu;
-                        const uint32_t hi = (c + 2 * i + 1 >= 0 && c + 2 * i + 1 < V) ? h[2 * i + 1] : kNegInf & 0xFFFFu;
-                        w[8 * j + i] = lo | (hi << 16);
-                    }
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (DT == ADA_F32) {
+                    w[i] = (c + i >= 0 && c + i < V) ? reinterpret_cast<const uint32_t*>(p)[i] : kNegInf;
+                } else {
+                    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+                    const uint32_t lo = (c + 2 * i >= 0 && c + 2 * i < V) ? h[2 * i] : kNegInf & 0xFFFFu;
+                    const uint32_t hi = (c + 2 * i + 1 >= 0 && c + 2 * i + 1 < V) ? h[2 * i + 1] : kNegInf & 0xFFFFu;
+                    w[i] = lo | (hi << 16);
                 }
             }
         }
     }
-    __device__ static void unpack(const uint32_t (&w)[NV * 8], float (&x)[kPer]) {
+    __device__ void load(int round, uint32_t (&w)[NV * 8]) const {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) vector(column(round, j), w + 8 * j);
+    }
+    template <int WORDS, int N>
+    __device__ static void unpack(const uint32_t (&w)[WORDS], float (&x)[N]) {
         if constexpr (DT == ADA_F32) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) x[i] = __uint_as_float(w[i]);
+            for (int i = 0; i < N; ++i) x[i] = __uint_as_float(w[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < kPer / 2; ++i) {
+            for (int i = 0; i < N / 2; ++i) {
                 if constexpr (DT == ADA_BF16) {
                     x[2 * i] = __uint_as_float(w[i] << 16);
                     x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
@@ -312,25 +309,34 @@ __device__ Sums plain_sums(const Reader<DT>& R, Sums* s_warp) {
 // ---- top k ---------------------------------------------------------------------------
 
 struct TopState {
-    uint64_t list[kWarps][kList];
+    uint64_t cand[kCand];
     uint64_t best[8 * kMaxTop];    // the row's best, then those of the cluster's other parts
     uint64_t sorted[kMaxTop];
-    float seen[kGroups];           // largest logit of a pair of threads so far
-    uint32_t bound;                // the highest bound found so far, as an order (0: none)
-    int count[kWarps];
-    int n_best;
+    float seen[kGroups];           // largest logit of a pair of threads
+    int count, n_best;
     uint32_t hist[256];
     uint32_t digit, below;
+};
+
+// Of a thread's rounds: the largest maximum, whose it is, and the second largest.
+struct Seen {
+    float top, second;
+    int round;
+    __device__ __forceinline__ void add(float x, int r) {
+        const bool more = !(x <= top);  // NaN too
+        second = max_nan(second, more ? top : x);
+        round = more ? r : round;
+        top = more ? x : top;
+    }
 };
 
 // Order of a value as an unsigned number (NaN above all).
 __device__ __forceinline__ uint32_t order_of(float x) { return static_cast<uint32_t>(key_of(x, 0) >> 32); }
 
 // The k-th largest of what groups of threads have seen, as an order rounded
-// down to its first 16 bits; 0 where that is not above the clamp. By one warp,
-// without a barrier: a value read too early is smaller and its bound holds all
-// the same. G groups per lane (32 G in all): more for larger k, as the k-th
-// largest of n groups' maxima has about n log(n / (n - k)) logits above it.
+// down to its first 16 bits; 0 where that is not above the clamp. G groups per
+// lane (32 G in all): more for larger k, as the k-th largest of n groups' maxima
+// has about n log(n / (n - k)) logits above it.
 template <int DT, int G>
 __device__ __forceinline__ uint32_t find_bound_of(const TopState& S, int k) {
     const int lane = threadIdx.x & 31;
@@ -340,7 +346,7 @@ __device__ __forceinline__ uint32_t find_bound_of(const TopState& S, int k) {
         float x = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4 / G; ++j)
-            x = max_nan(x, *const_cast<const volatile float*>(&S.seen[(i * (4 / G) + j) * 32 + lane]));
+            x = max_nan(x, S.seen[(i * (4 / G) + j) * 32 + lane]);
         v[i] = order_of(x);
     }
     uint32_t prefix = 0;
@@ -359,140 +365,136 @@ __device__ uint32_t find_bound(const TopState& S, int k) {
     return k <= 8 ? find_bound_of<DT, 1>(S, k) : k <= 24 ? find_bound_of<DT, 2>(S, k) : find_bound_of<DT, 4>(S, k);
 }
 
-// Cuts a warp's list of n > k keys to its k best and returns the smallest of
-// them: the k-th largest key, bit by bit.
-__device__ uint64_t cut_list(uint64_t* list, int n, int k) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-    uint64_t prefix = 0;
-#pragma unroll 1
-    for (int b = 63; b >= 0; --b) {
-        const uint64_t c = prefix | (uint64_t(1) << b);
-        int have = 0;
-        for (int i = lane; i - lane < n; i += 32) have += __popc(__ballot_sync(0xffffffffu, i < n && list[i] >= c));
-        if (have >= k) prefix = c;
-    }
-    int kept = 0;
-    for (int i = lane; i - lane < n; i += 32) {  // kept <= i: nothing unread is overwritten
-        const uint64_t key = i < n ? list[i] : 0;
-        const bool take = i < n && key >= prefix;
-        const uint32_t who = __ballot_sync(0xffffffffu, take);
-        if (take) list[kept + __popc(who & ((1u << lane) - 1u))] = key;
-        kept += __popc(who);
-        __syncwarp();
-    }
-    return prefix;
-}
-
 // The k best keys of the first n of best[] (n <= 512), in order, to sorted[].
 __device__ void sort_best(TopState& S, int n, int k) {
     for (int i = threadIdx.x; i < n; i += kT) {
         const uint64_t mine = S.best[i];
         int r = 0;
+#pragma unroll 8
         for (int j = 0; j < n; ++j) r += S.best[j] > mine;
         if (r < k) S.sorted[r] = mine;
     }
     __syncthreads();
 }
 
-// The block's k best keys (all it has, when fewer), in order, to sorted[].
-template <int DT>
-__device__ void gather_best(TopState& S, int k) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) S.n_best = 0;
-    __syncthreads();
-    uint64_t from = static_cast<uint64_t>(S.bound) << 32;
-    const int len = S.count[warp];
-    int mine = 0;
-    for (int i = lane; i < len; i += 32) mine += S.list[warp][i] >= from;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) atomicAdd(&S.n_best, mine);
-    __syncthreads();
-    const int n = S.n_best;
-    __syncthreads();
-    if (threadIdx.x == 0) S.n_best = 0;
-    if (n > 8 * kMaxTop) {  // many equal logits: the exact k-th largest key, a byte at a time
-        uint64_t prefix = 0, mask = 0;
-        int want = k;
-        for (int b = 56; b >= 0; b -= 8) {
-            S.hist[threadIdx.x] = 0;
-            __syncthreads();
-            for (int i = lane; i < len; i += 32) {
-                const uint64_t key = S.list[warp][i];
-                if ((key & mask) == prefix) atomicAdd(&S.hist[(key >> b) & 255u], 1u);
-            }
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                int d = 255, before = 0;
-                while (d > 0 && before + static_cast<int>(S.hist[d]) < want) before += static_cast<int>(S.hist[d--]);
-                S.digit = static_cast<uint32_t>(d);
-                S.below = static_cast<uint32_t>(before);
-            }
-            __syncthreads();
-            prefix |= static_cast<uint64_t>(S.digit) << b;
-            mask |= uint64_t(255) << b;
-            want -= static_cast<int>(S.below);
+// Adds one to the digit's bin for every lane that takes part; lanes that share
+// the first one's digit (all of them in a constant row) add up first.
+__device__ __forceinline__ void count_digit(TopState& S, bool on, uint32_t digit) {
+    const uint32_t active = __ballot_sync(0xffffffffu, on);
+    if (active == 0) return;
+    const int first = __ffs(active) - 1;
+    const uint32_t shared = __shfl_sync(0xffffffffu, digit, first);  // every lane takes part in the exchange
+    const bool same = on && digit == shared;
+    const uint32_t together = __ballot_sync(0xffffffffu, same);
+    if (same) {
+        if (static_cast<int>(threadIdx.x & 31) == first) atomicAdd(&S.hist[digit], static_cast<uint32_t>(__popc(together)));
+    } else if (on) {
+        atomicAdd(&S.hist[digit], 1u);
+    }
+}
+
+// The k-th largest of a set of keys, a byte at a time; each(f) calls f(key, on)
+// for all of them, whole warps at a time. 0 when there are fewer than k.
+template <class Each>
+__device__ uint64_t select_key(TopState& S, int k, const Each& each) {
+    uint64_t prefix = 0, mask = 0;
+    int want = k;
+    for (int b = 56; b >= 0; b -= 8) {
+        __syncthreads();
+        S.hist[threadIdx.x] = 0;
+        __syncthreads();
+        each([&](uint64_t key, bool on) {
+            count_digit(S, on && (key & mask) == prefix, static_cast<uint32_t>(key >> b) & 255u);
+        });
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int d = 255, before = 0;
+            while (d > 0 && before + static_cast<int>(S.hist[d]) < want) before += static_cast<int>(S.hist[d--]);
+            S.digit = static_cast<uint32_t>(d);
+            S.below = static_cast<uint32_t>(before);
         }
-        from = prefix;
+        __syncthreads();
+        prefix |= static_cast<uint64_t>(S.digit) << b;
+        mask |= uint64_t(255) << b;
+        want -= static_cast<int>(S.below);
+    }
+    return prefix;
+}
+
+// The k best keys of this block's rounds of the row (all, when it has fewer),
+// in order, to sorted[].
+template <int DT>
+__device__ void best_keys(TopState& S, int k, const Seen& mine, const Reader<DT>& R, int rank, int parts) {
+    constexpr int EPV = Reader<DT>::EPV, NV = Reader<DT>::NV;
+    const int lane = threadIdx.x & 31;
+    const float pair = max_nan(mine.top, __shfl_xor_sync(0xffffffffu, mine.top, 1));
+    if ((lane & 1) == 0) S.seen[threadIdx.x >> 1] = pair;
+    if (threadIdx.x == 0) S.count = S.n_best = 0;
+    __syncthreads();
+    const uint32_t bound = find_bound<DT>(S, k);
+    const int rounds = R.rounds();
+    const int vectors = rank < rounds ? ((rounds - rank + parts - 1) / parts) * NV : 0;  // of each thread
+    if (bound != 0) {
+        // the keys of the vector at column c that reach the bound
+        auto take = [&](int c) {
+            uint32_t w[8];
+            float x[EPV];
+            R.vector(c, w);
+            Reader<DT>::unpack(w, x);
+#pragma unroll
+            for (int i = 0; i < EPV; ++i) {
+                if (c + i < 0 || c + i >= R.V || order_of(x[i]) < bound) continue;
+                const int at = atomicAdd(&S.count, 1);
+                if (at < kCand) S.cand[at] = key_of(x[i], c + i);
+            }
+        };
+        if (order_of(mine.top) >= bound)
+            for (int j = 0; j < NV; ++j) take(R.column(mine.round, j));
+        __syncwarp();
+        for (uint32_t todo = __ballot_sync(0xffffffffu, order_of(mine.second) >= bound); todo != 0; todo &= todo - 1) {
+            const int who = __ffs(todo) - 1;
+            const int done = __shfl_sync(0xffffffffu, mine.round, who);
+            for (int v = lane; v < vectors; v += 32) {
+                const int round = rank + (v / NV) * parts;
+                if (round != done) take(R.column(round, v % NV) + (who - lane) * EPV);
+            }
+            __syncwarp();
+        }
     }
     __syncthreads();
-    for (int i = lane; i < len; i += 32) {
-        const uint64_t key = S.list[warp][i];
-        if (key >= from) S.best[atomicAdd(&S.n_best, 1)] = key;
+    const int n = S.count;
+    if (bound == 0 || n > kCand) {  // too many equal logits, or too few above the clamp: all keys of the rounds
+        auto each = [&](auto&& f) {
+            for (int r = rank; r < rounds; r += parts) {
+                uint32_t w[NV * 8];
+                float x[kPer];
+                R.load(r, w);
+                Reader<DT>::unpack(w, x);
+#pragma unroll 4
+                for (int i = 0; i < kPer; ++i) {
+                    const int c = R.column(r, i / EPV) + i % EPV;
+                    f(key_of(x[i], c), c >= 0 && c < R.V);
+                }
+            }
+        };
+        const uint64_t from = select_key(S, k, each);
+        each([&](uint64_t key, bool on) {
+            if (on && key >= from) S.best[atomicAdd(&S.n_best, 1)] = key;
+        });
+    } else {
+        uint64_t from = 0;
+        if (n > 8 * kMaxTop) {
+            from = select_key(S, k, [&](auto&& f) {
+                for (int i = threadIdx.x; i - lane < n; i += kT) f(i < n ? S.cand[i] : 0, i < n);
+            });
+        }
+        for (int i = threadIdx.x; i < n; i += kT)
+            if (S.cand[i] >= from) S.best[atomicAdd(&S.n_best, 1)] = S.cand[i];
     }
     __syncthreads();
     sort_best(S, S.n_best, k);
     if (threadIdx.x == 0) S.n_best = min(S.n_best, k);
     __syncthreads();
-}
-
-// One round's elements for the lists. `seen`: the largest logit this thread
-// has met; `exact`: keys below it are out of this warp's k best.
-template <int DT>
-__device__ __forceinline__ void top_round(TopState& S, int k, const uint32_t (&w)[Reader<DT>::NV * 8], float top, float& seen,
-                                          uint64_t& exact, int turn, const Reader<DT>& R, int round) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    seen = max_nan(seen, top);
-    if ((turn & (turn + 1)) == 0) {  // 0, 1, 3, 7, ...
-        const float pair = max_nan(seen, __shfl_xor_sync(0xffffffffu, seen, 1));
-        if ((lane & 1) == 0) *const_cast<volatile float*>(&S.seen[threadIdx.x >> 1]) = pair;
-        if (turn == 0) __syncthreads();
-        __syncwarp();
-        if (warp == (turn & (kWarps - 1))) {
-            const uint32_t b = find_bound<DT>(S, k);
-            if (lane == 0) atomicMax(&S.bound, b);
-            __syncwarp();
-        }
-        if (turn == 0) __syncthreads();
-    }
-    if (!R.any(round)) return;
-    const uint32_t bound = *const_cast<const volatile uint32_t*>(&S.bound);
-    const float low = bound == 0u ? -INFINITY : value_of(static_cast<uint64_t>(bound) << 32);
-    if (__any_sync(0xffffffffu, !(top < low))) {
-        float x[kPer];
-        Reader<DT>::unpack(w, x);
-        int n = S.count[warp];
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            constexpr int EPV = Reader<DT>::EPV;
-            const int c = R.column(round, i / EPV) + i % EPV;
-            if (__any_sync(0xffffffffu, !(x[i] < low))) {
-                const uint64_t key = key_of(x[i], c);
-                const bool take = (key >> 32) >= bound && key >= exact && c >= 0 && c < R.V;
-                const uint32_t who = __ballot_sync(0xffffffffu, take);
-                if (take) S.list[warp][n + __popc(who & ((1u << lane) - 1u))] = key;
-                n += __popc(who);
-            }
-            if ((i + 1) % (kPer / 2) == 0 && n > kMark) {
-                exact = cut_list(S.list[warp], n, k);
-                n = k;
-            }
-        }
-        __syncwarp();
-        if (lane == 0) S.count[warp] = n;
-        __syncwarp();
-    }
 }
 
 // ---- forward -------------------------------------------------------------------------
@@ -511,24 +513,18 @@ __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constan
     const uint8_t* zr = static_cast<const uint8_t*>(L.logits) + off * EB;
     const Reader<DT> R(zr, L.V);
     const int k = TOP ? L.top : 0;
-    if constexpr (TOP) {
-        if (threadIdx.x < kGroups) S.seen[threadIdx.x] = -INFINITY;
-        if (threadIdx.x < kWarps) S.count[threadIdx.x] = 0;
-        if (threadIdx.x == 0) S.bound = 0;
-        __syncthreads();
-    }
     PairSums sums{-INFINITY, f2_splat(0.f), f2_splat(0.f)};
-    float seen = -INFINITY;
-    uint64_t exact = 0;
+    Seen seen{-INFINITY, -INFINITY, 0};
     const int rounds = R.rounds();
     uint32_t w[Reader<DT>::NV * 8], next[Reader<DT>::NV * 8];
     if (rank < rounds) R.load(rank, w);
-    int turn = 0;
-    for (int r = rank; r < rounds; r += parts, ++turn) {
+#pragma unroll 2
+    for (int r = rank; r < rounds; r += parts) {
         if (r + parts < rounds) R.load(r + parts, next);
-        float top = -INFINITY;
-        if (R.any(r)) top = add_round<DT>(sums, w);
-        if constexpr (TOP) top_round<DT>(S, k, w, top, seen, exact, turn, R, r);
+        if (R.any(r)) {
+            const float top = add_round<DT>(sums, w);
+            if (TOP) seen.add(top, r);
+        }
 #pragma unroll
         for (int j = 0; j < Reader<DT>::NV * 8; ++j) w[j] = next[j];
     }
@@ -545,7 +541,7 @@ __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constan
         a = join_warp(threadIdx.x < kWarps ? s_warp[threadIdx.x] : Sums{-INFINITY, 0.f, 0.f}, kWarps);
         if (threadIdx.x == 0) s_part = a;
     }
-    if constexpr (TOP) gather_best<DT>(S, k);
+    if constexpr (TOP) best_keys<DT>(S, k, seen, R, rank, parts);
     if (parts > 1) {
         cluster.sync();
         if (rank == 0) {
