@@ -568,9 +568,14 @@ int ada_token_logprobs(const AdaTensor* logits, const AdaTensor* tokens, int64_t
     L.stats = stats;
     L.top_logprobs = top_logprobs;
     L.top_tokens = top_tokens;
-    L.cluster = 1;
     if (L.rows * 8 > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "too many rows");
-    if ((rc = device_status_word(&L.status))) return rc;
+    int sms;
+    if ((rc = device_status_word(&L.status)) || (rc = sm_count(&sms))) return rc;
+    // Few rows: a cluster of up to 8 CTAs per row, while the CTAs are at most
+    // two per SM and each still has a round of 4096 logits.
+    L.cluster = 1;
+    const int64_t rounds = (L.V + 4095) / 4096;
+    while (L.cluster < 8 && L.rows * L.cluster * 2 <= 2 * sms && L.cluster * 2 <= rounds) L.cluster *= 2;
     rc = launch_token_logprobs(L, static_cast<cudaStream_t>(stream));
     return rc ? fail(rc, "token log-probability launch failed: %s", cudaGetErrorString(cudaGetLastError())) : ADA_OK;
 }
@@ -595,9 +600,13 @@ int ada_token_logprobs_bwd(const AdaTensor* logits, const AdaTensor* tokens, int
     L.grad = grad->data;
     L.gs0 = row_stride(grad, 0);
     L.gs1 = row_stride(grad, 1);
-    L.segments = 1;
-    if (L.rows * 64 > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "too many rows");
-    if ((rc = device_status_word(&L.status))) return rc;
+    if (L.rows * 8 > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "too many rows");
+    int sms;
+    if ((rc = device_status_word(&L.status)) || (rc = sm_count(&sms))) return rc;
+    // Blocks to fill the GPU eight deep, of at least a round of 4096 logits each.
+    const int64_t rounds = (L.V + 4095) / 4096;
+    L.segments = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(rounds, (int64_t(sms) * 8 + L.rows - 1) / L.rows)));
+    if (L.rows * L.segments > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "too many rows");
     rc = launch_token_logprobs_bwd(L, static_cast<cudaStream_t>(stream));
     return rc ? fail(rc, "token log-probability gradient launch failed: %s", cudaGetErrorString(cudaGetLastError())) : ADA_OK;
 }

@@ -24,12 +24,12 @@
 //
 // Top k (k <= 64): candidates are 64-bit keys, the value's order above the
 // inverted column, so all keys differ and equal values rank by lowest index.
-// While the row is read, a thread only keeps the largest logit it has seen,
-// the vector that held it, and the second largest of its vectors' maxima. The
-// k-th largest of 128 thread pairs' maxima bounds the k-th best logit from
-// below, and what reaches it lies with the few threads (about k) whose maximum
-// does: each reads that one vector again (L2), and the rare thread whose second
-// vector reaches the bound too has all its vectors read by its warp. The logits
+// While the row is read, a thread only keeps the maxima of its two best rounds,
+// which they were, and the third largest maximum. The k-th largest of 128
+// thread pairs' maxima bounds the k-th best logit from below, and what reaches
+// it lies with the few threads (about k) whose maximum does: each reads those
+// rounds again (L2), and the rare thread with a third round at the bound has
+// all its rounds read by its warp. The logits
 // at or above the bound are sorted. A row with more of them than fit (masked or
 // constant rows) takes radix passes over all its keys instead.
 #include <cooperative_groups.h>
@@ -63,6 +63,11 @@ __device__ __forceinline__ uint64_t key_of(float x, int col) {
     const uint32_t b = __float_as_uint(x + 0.f);  // -0 ranks as 0
     const uint32_t o = isnan(x) ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
     return (static_cast<uint64_t>(o) << 32) | (0xFFFFFFFFu - static_cast<uint32_t>(col));
+}
+// Its value (0 for -0).
+__device__ __forceinline__ float value_of(uint64_t key) {
+    const uint32_t o = static_cast<uint32_t>(key >> 32);
+    return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
 __device__ __forceinline__ int column_of(uint64_t key) {
     return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key));
@@ -318,51 +323,56 @@ struct TopState {
     uint32_t digit, below;
 };
 
-// Of a thread's rounds: the largest maximum, whose it is, and the second largest.
+// Of a thread's rounds: the three largest maxima and the rounds of the first two.
 struct Seen {
-    float top, second;
-    int round;
+    float top, second, third;
+    int round, round2;
     __device__ __forceinline__ void add(float x, int r) {
-        const bool more = !(x <= top);  // NaN too
-        second = max_nan(second, more ? top : x);
-        round = more ? r : round;
-        top = more ? x : top;
+        const bool first = !(x <= top), next = !(x <= second);  // NaN too
+        third = max_nan(third, next ? second : x);
+        second = first ? top : next ? x : second;
+        round2 = first ? round : next ? r : round2;
+        top = first ? x : top;
+        round = first ? r : round;
     }
 };
 
 // Order of a value as an unsigned number (NaN above all).
 __device__ __forceinline__ uint32_t order_of(float x) { return static_cast<uint32_t>(key_of(x, 0) >> 32); }
 
-// The k-th largest of what groups of threads have seen, as an order rounded
-// down to its first 16 bits; 0 where that is not above the clamp. G groups per
-// lane (32 G in all): more for larger k, as the k-th largest of n groups' maxima
-// has about n log(n / (n - k)) logits above it.
-template <int DT, int G>
-__device__ __forceinline__ uint32_t find_bound_of(const TopState& S, int k) {
-    const int lane = threadIdx.x & 31;
-    uint32_t v[G];
-#pragma unroll
-    for (int i = 0; i < G; ++i) {
-        float x = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 4 / G; ++j)
-            x = max_nan(x, S.seen[(i * (4 / G) + j) * 32 + lane]);
-        v[i] = order_of(x);
-    }
-    uint32_t prefix = 0;
-#pragma unroll 1
-    for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
-        const uint32_t c = prefix | bit;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < G; ++i) n += __popc(__ballot_sync(0xffffffffu, v[i] >= c));
-        if (n >= k) prefix = c;
-    }
-    return prefix <= order_of(lowest_kept<DT>()) ? 0u : prefix;
-}
+// A lower bound of the k-th best logit, as an order; 0 where that is not above
+// the clamp: the k-th largest of the maxima of 32 groups of threads (k <= 24;
+// sorted across the lanes) or of 128 pairs (to the first 16 bits of its order,
+// a bit at a time). The k-th largest of n groups' maxima has about
+// n log(n / (n - k)) logits above it.
 template <int DT>
 __device__ uint32_t find_bound(const TopState& S, int k) {
-    return k <= 8 ? find_bound_of<DT, 1>(S, k) : k <= 24 ? find_bound_of<DT, 2>(S, k) : find_bound_of<DT, 4>(S, k);
+    const int lane = threadIdx.x & 31;
+    uint32_t v[kGroups / 32], found = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups / 32; ++i) v[i] = order_of(S.seen[i * 32 + lane]);
+    if (k <= 24) {
+        uint32_t x = max(max(v[0], v[1]), max(v[2], v[3]));
+#pragma unroll
+        for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+            for (int o = n >> 1; o > 0; o >>= 1) {
+                const uint32_t y = __shfl_xor_sync(0xffffffffu, x, o);
+                const bool down = (lane & n) == 0 || n == 32;  // this run is sorted downwards
+                x = (((lane & o) == 0) == down) ? max(x, y) : min(x, y);
+            }
+        found = __shfl_sync(0xffffffffu, x, k - 1);
+    } else {
+#pragma unroll 1
+        for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+            const uint32_t c = found | bit;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < kGroups / 32; ++i) n += __popc(__ballot_sync(0xffffffffu, v[i] >= c));
+            if (n >= k) found = c;
+        }
+    }
+    return found <= order_of(lowest_kept<DT>()) ? 0u : found;
 }
 
 // The k best keys of the first n of best[] (n <= 512), in order, to sorted[].
@@ -435,28 +445,56 @@ __device__ void best_keys(TopState& S, int k, const Seen& mine, const Reader<DT>
     const int rounds = R.rounds();
     const int vectors = rank < rounds ? ((rounds - rank + parts - 1) / parts) * NV : 0;  // of each thread
     if (bound != 0) {
-        // the keys of the vector at column c that reach the bound
-        auto take = [&](int c) {
-            uint32_t w[8];
-            float x[EPV];
-            R.vector(c, w);
-            Reader<DT>::unpack(w, x);
+        // A warp takes its threads at the bound four at a time: half of the lanes
+        // read the elements of the best round, the others those of the second.
+        const int half = lane >> 4, e = lane & 15;
+        const int at = (e / EPV) * kT * EPV + e % EPV - lane * EPV + R.c0;
+        uint32_t todo = __ballot_sync(0xffffffffu, order_of(mine.top) >= bound);
+        const uint32_t more = __ballot_sync(0xffffffffu, order_of(mine.second) >= bound);
+        while (todo != 0) {
+            float x[4];
+            int c[4];
 #pragma unroll
-            for (int i = 0; i < EPV; ++i) {
-                if (c + i < 0 || c + i >= R.V || order_of(x[i]) < bound) continue;
-                const int at = atomicAdd(&S.count, 1);
-                if (at < kCand) S.cand[at] = key_of(x[i], c + i);
+            for (int u = 0; u < 4; ++u) {
+                c[u] = -1;
+                x[u] = -INFINITY;
+                if (todo == 0) continue;
+                const int who = __ffs(todo) - 1;
+                todo &= todo - 1;
+                const int r1 = __shfl_sync(0xffffffffu, mine.round, who), r2 = __shfl_sync(0xffffffffu, mine.round2, who);
+                if (half == 0 || ((more >> who) & 1u)) c[u] = (half == 0 ? r1 : r2) * kRound + who * EPV + at;
+                if (c[u] >= 0 && c[u] < R.V) x[u] = load_as_f32(R.mine, c[u] - R.c0, DT);
             }
-        };
-        if (order_of(mine.top) >= bound)
-            for (int j = 0; j < NV; ++j) take(R.column(mine.round, j));
-        __syncwarp();
-        for (uint32_t todo = __ballot_sync(0xffffffffu, order_of(mine.second) >= bound); todo != 0; todo &= todo - 1) {
-            const int who = __ffs(todo) - 1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool ok = c[u] >= 0 && c[u] < R.V && order_of(x[u]) >= bound;
+                const uint32_t oks = __ballot_sync(0xffffffffu, ok);
+                if (oks == 0) continue;
+                int base = 0;
+                if (lane == 0) base = atomicAdd(&S.count, __popc(oks));
+                base = __shfl_sync(0xffffffffu, base, 0) + __popc(oks & ((1u << lane) - 1u));
+                if (ok && base < kCand) S.cand[base] = key_of(x[u], c[u]);
+            }
+        }
+        // further rounds of a thread, a lane for each vector
+        for (uint32_t rare = __ballot_sync(0xffffffffu, order_of(mine.third) >= bound); rare != 0; rare &= rare - 1) {
+            const int who = __ffs(rare) - 1;
             const int done = __shfl_sync(0xffffffffu, mine.round, who);
+            const int done2 = __shfl_sync(0xffffffffu, mine.round2, who);
             for (int v = lane; v < vectors; v += 32) {
                 const int round = rank + (v / NV) * parts;
-                if (round != done) take(R.column(round, v % NV) + (who - lane) * EPV);
+                if (round == done || round == done2) continue;
+                const int col = R.column(round, v % NV) + (who - lane) * EPV;
+                uint32_t w[8];
+                float x[EPV];
+                R.vector(col, w);
+                Reader<DT>::unpack(w, x);
+#pragma unroll
+                for (int i = 0; i < EPV; ++i) {
+                    if (col + i < 0 || col + i >= R.V || order_of(x[i]) < bound) continue;
+                    const int slot = atomicAdd(&S.count, 1);
+                    if (slot < kCand) S.cand[slot] = key_of(x[i], col + i);
+                }
             }
             __syncwarp();
         }
@@ -492,15 +530,15 @@ __device__ void best_keys(TopState& S, int k, const Seen& mine, const Reader<DT>
             if (S.cand[i] >= from) S.best[atomicAdd(&S.n_best, 1)] = S.cand[i];
     }
     __syncthreads();
-    sort_best(S, S.n_best, k);
-    if (threadIdx.x == 0) S.n_best = min(S.n_best, k);
-    __syncthreads();
+    const int have = S.n_best;
+    if (static_cast<int>(threadIdx.x) >= have && static_cast<int>(threadIdx.x) < k) S.sorted[threadIdx.x] = 0;  // below any key
+    sort_best(S, have, k);
 }
 
 // ---- forward -------------------------------------------------------------------------
 
 template <int DT, bool TOP>
-__global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constant__ LogprobLaunch L) {
+__global__ void __launch_bounds__(kT, DT == ADA_F32 ? 0 : TOP ? 6 : 8) token_logprobs_kernel(const __grid_constant__ LogprobLaunch L) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Sums s_warp[kWarps];
     __shared__ Sums s_part;
@@ -513,8 +551,16 @@ __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constan
     const uint8_t* zr = static_cast<const uint8_t*>(L.logits) + off * EB;
     const Reader<DT> R(zr, L.V);
     const int k = TOP ? L.top : 0;
+    // the given token's logit is on its way while the row is read
+    float zt = 0.f;
+    int token = 0;  // 1: ignored, 2: outside the vocabulary
+    if (rank == 0 && threadIdx.x == 0) {
+        const int64_t t = L.tok64 ? static_cast<const int64_t*>(L.tokens)[row] : static_cast<const int32_t*>(L.tokens)[row];
+        token = t == L.ignore ? 1 : (t < 0 || t >= L.V) ? 2 : 0;
+        if (token == 0) zt = load_as_f32(zr, t, DT);
+    }
     PairSums sums{-INFINITY, f2_splat(0.f), f2_splat(0.f)};
-    Seen seen{-INFINITY, -INFINITY, 0};
+    Seen seen{-INFINITY, -INFINITY, -INFINITY, 0, 0};
     const int rounds = R.rounds();
     uint32_t w[Reader<DT>::NV * 8], next[Reader<DT>::NV * 8];
     if (rank < rounds) R.load(rank, w);
@@ -552,15 +598,10 @@ __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constan
                 if (threadIdx.x == 0) s_part = a;
             }
             if constexpr (TOP) {
-                int n = 0;
-                for (int i = 0; i < parts; ++i) {
-                    const TopState* T = cluster.map_shared_rank(&S, i);
-                    const int m = T->n_best;
-                    for (int j = threadIdx.x; j < m; j += kT) S.best[n + j] = T->sorted[j];
-                    n += m;
-                }
+                for (int i = threadIdx.x; i < parts * k; i += kT)
+                    S.best[i] = cluster.map_shared_rank(&S, i / k)->sorted[i % k];
                 __syncthreads();
-                sort_best(S, n, k);
+                sort_best(S, parts * k, k);
             }
         }
         cluster.sync();  // the parts stay until they are read
@@ -581,15 +622,10 @@ __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constan
         mean = (a.t / a.s - r) * kLn2;
     }
     if (threadIdx.x == 0) {
-        const int64_t t = L.tok64 ? static_cast<const int64_t*>(L.tokens)[row] : static_cast<const int32_t*>(L.tokens)[row];
-        float lp = 0.f;
-        if (t != L.ignore) {
-            if (t >= 0 && t < L.V) {
-                lp = (load_as_f32(zr, t, DT) - a.m) - ls;
-            } else {
-                lp = __int_as_float(0x7FFFFFFF);
-                record_error(L.status, ADA_ERR_INVALID);
-            }
+        float lp = token == 0 ? (zt - a.m) - ls : 0.f;
+        if (token == 2) {
+            lp = __int_as_float(0x7FFFFFFF);
+            record_error(L.status, ADA_ERR_INVALID);
         }
         L.logprobs[row] = lp;
         L.entropy[row] = ls - mean;
@@ -601,7 +637,7 @@ __global__ void __launch_bounds__(kT) token_logprobs_kernel(const __grid_constan
         for (int i = threadIdx.x; i < k; i += kT) {
             const int c = column_of(S.sorted[i]);
             L.top_tokens[row * k + i] = c;
-            L.top_logprobs[row * k + i] = (load_as_f32(zr, c, DT) - a.m) - ls;
+            L.top_logprobs[row * k + i] = (value_of(S.sorted[i]) - a.m) - ls;
         }
     }
 }
