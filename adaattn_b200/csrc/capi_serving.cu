@@ -455,10 +455,12 @@ int ada_paged_append(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages,
     L.k_scale = given(k_scale) ? static_cast<const float*>(k_scale->data) : nullptr;
     L.v_scale = given(v_scale) ? static_cast<const float*>(v_scale->data) : nullptr;
     L.status = st;
-    // A block per 256 items of a sequence, and no more than fill the GPU eight times.
-    const int64_t items = N * Hkv * (L.vec ? D / 8 : D);
-    const int64_t most = std::max<int64_t>(1, int64_t(sms) * 64 / B);
-    L.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, most)));
+    // Blocks of 256 items (of whole tokens), and no more than fill the GPU twice.
+    const int64_t in_token = Hkv * (L.vec ? D / 8 : D);
+    if (in_token > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "too many heads");
+    const int64_t at_once = in_token < 256 ? 256 / in_token : 1;
+    const int64_t most = std::max<int64_t>(1, int64_t(sms) * 16 / B);
+    L.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((N + at_once - 1) / at_once, most)));
     if (B * L.chunks > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "too many sequences");
     rc = launch_paged_append(L, static_cast<cudaStream_t>(stream));
     return rc ? fail(rc, "append launch failed: %s", cudaGetErrorString(cudaGetLastError())) : ADA_OK;
