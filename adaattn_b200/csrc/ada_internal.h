@@ -321,6 +321,7 @@ struct PagedAttnLaunch {
     const int32_t* seqs;   // [B] table rows, or null: row b
     int64_t S, W, P, table_ld;
     int page;
+    uint32_t page_inv;   // ceil(2^32 / page); 0: page is 1
     MaskView mask;       // [B, mask_len] strides s[0], s[1]; keys from mask_len on are open
     int64_t mask_len;
     const float* k_scale;  // [Hkv] or null

@@ -354,6 +354,7 @@ int ada_paged_attn(const AdaTensor* q, const AdaTensor* k_pages, const AdaTensor
     L.table_ld = row_stride(page_table, 0);
     L.P = k_pages->shape[0];
     L.page = static_cast<int>(page);
+    L.page_inv = page == 1 ? 0u : static_cast<uint32_t>(((uint64_t(1) << 32) + page - 1) / page);
     if (given(key_mask)) {
         L.mask.data = key_mask->data;
         L.mask.dtype = key_mask->dtype;

@@ -12,7 +12,10 @@
 // So the work is split evenly over the cache, not over sequences: the tiles of
 // 32 keys of all (sequence, head block) units stand in one line, CTA c takes
 // the c-th equal piece of it and each of its warps an equal piece of that. A
-// unit that lies in one warp's piece is finished there. Pieces of a unit that
+// unit begins with kLead empty places, which stand for what a warp spends to
+// start and finish one (without them a warp with eight two-tile units ran four
+// times as long as the others). A unit that lies in one warp's piece is
+// finished there. Pieces of a unit that
 // spans warps are joined in shared memory (each with its running maximum m,
 // sum l and unnormalised accumulator), pieces that span CTAs are joined by a
 // second kernel. The split depends on the lengths alone, so results repeat.
@@ -25,7 +28,9 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;       // keys per tile
+constexpr int kLead = 3;        // places before a unit's tiles
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 // ---- the line of tiles -------------------------------------------------------
 
@@ -51,14 +56,15 @@ __device__ __forceinline__ int seq_length(const PagedAttnLaunch& L, int b) {
     return n;
 }
 
-// pref[b] = tiles of the sequences before b, pref[B] = all (every thread of the block calls it).
+// pref[b] = places per unit of the sequences before b, pref[B] = of all (every thread of the block calls it).
 __device__ void tile_prefix(const PagedAttnLaunch& L, int* pref, int* warp_sums) {
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
     const int per = (L.B + nt - 1) / nt;
     const int b0 = min(tid * per, L.B), b1 = min(b0 + per, L.B);
     int sum = 0;
     for (int b = b0; b < b1; ++b) {
-        const int n = (seq_length(L, b) + kTile - 1) / kTile;
+        const int tiles = (seq_length(L, b) + kTile - 1) / kTile;
+        const int n = tiles > 0 ? tiles + kLead : 0;
         pref[b] = n;
         sum += n;
     }
@@ -87,6 +93,7 @@ struct Unit {
     int64_t t0, t1;  // its tiles on the line
 };
 
+// The unit whose tiles or leading places hold place t.
 __device__ __forceinline__ Unit unit_at(const PagedAttnLaunch& L, const int* pref, int64_t t) {
     const int q = static_cast<int>(t / L.U);
     int lo = 0, hi = L.B - 1;
@@ -100,15 +107,28 @@ __device__ __forceinline__ Unit unit_at(const PagedAttnLaunch& L, const int* pre
     const int64_t first = static_cast<int64_t>(pref[lo]) * L.U;
     const int n = pref[lo + 1] - pref[lo];
     x.u = static_cast<int>((t - first) / n);
-    x.t0 = first + static_cast<int64_t>(x.u) * n;
+    x.t0 = first + static_cast<int64_t>(x.u) * n + kLead;
+    x.t1 = x.t0 + n - kLead;
+    return x;
+}
+
+// The unit after x; t0 past the line's end when there is none.
+__device__ __forceinline__ Unit unit_after(const PagedAttnLaunch& L, const int* pref, Unit x) {
+    const int64_t n = x.t1 - x.t0;
+    x.t0 = x.t1 + kLead;
     x.t1 = x.t0 + n;
+    if (++x.u < L.U) return x;
+    x.u = 0;
+    do ++x.b;
+    while (x.b < L.B && pref[x.b + 1] == pref[x.b]);
+    if (x.b < L.B) x.t1 = x.t0 + (pref[x.b + 1] - pref[x.b] - kLead);
     return x;
 }
 
 // The CTAs that take part and the piece of CTA c: [c T / n, (c + 1) T / n).
 __device__ __forceinline__ int64_t pieces(int64_t T, int64_t most) { return T < most ? T : most; }
 __device__ __forceinline__ int64_t piece_start(int64_t c, int64_t T, int64_t n) { return c * T / n; }
-// The piece that holds tile t.
+// The piece that holds place t.
 __device__ __forceinline__ int64_t piece_of(int64_t t, int64_t T, int64_t n) { return ((t + 1) * n - 1) / T; }
 
 // ---- element access ----------------------------------------------------------
@@ -254,7 +274,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     if (c0 + 1 >= nc) return;
     const int64_t edge = piece_start(c0 + 1, T, nc);
     const Unit x = unit_at(L, L.pref, edge);
-    if (x.t0 == edge || piece_of(x.t0, T, nc) != c0) return;
+    if (x.t0 >= edge || piece_of(x.t0, T, nc) != c0) return;
     const int g = x.u / L.HB, h0 = g * L.G + (x.u % L.HB) * L.GB;
     if (h >= min(L.GB, (g + 1) * L.G - h0)) return;
     const int n = static_cast<int>(piece_of(x.t1 - 1, T, nc) - c0 + 1);
@@ -340,8 +360,8 @@ __global__ void __launch_bounds__(kThreads) paged_simt_kernel(const __grid_const
     int64_t t = ca + (cz - ca) * warp / kWarps;
     const int64_t a = t, z = ca + (cz - ca) * (warp + 1) / kWarps;
     const int kg = lane / LPK, c0 = (lane & (LPK - 1)) * 4;
-    while (t < z) {
-        const Unit x = unit_at(L, pref, t);
+    for (Unit x = t < z ? unit_at(L, pref, t) : Unit{0, 0, z, z}; x.t0 < z; x = unit_after(L, pref, x)) {
+        if (t < x.t0) t = x.t0;
         const int64_t tz = x.t1 < z ? x.t1 : z;
         const int g = x.u / L.HB, h0 = g * L.G + (x.u % L.HB) * GB;
         const int heads = min(GB, (g + 1) * L.G - h0);
@@ -531,7 +551,9 @@ struct TcCfg {
     static constexpr int NBOX = D * EB / RB;
     static constexpr int HALF = kTile * D * EB;              // K or V bytes of a tile
     static constexpr int TILE = 2 * HALF;
-    static constexpr int WARPS = TILE >= 16384 ? 4 : 8;
+    // 8-bit pages of 128 elements are bound by the instructions between their
+    // bytes, which more warps overlap: 10 of 2 stages instead of 8 of 3.
+    static constexpr int WARPS = TILE >= 16384 ? 4 : (KIND == 2 && D == 128 && NT == 1) ? 10 : 8;
     static constexpr int STAGES = TILE >= 8192 ? 3 : 6;      // at most; fewer when the rest needs the space
     static constexpr int GB = 8 * NT;
     static constexpr int PART = GB * D;                      // floats a warp leaves per slot
@@ -542,11 +564,11 @@ struct TcCfg {
 template <int KIND>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (KIND == 0)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -560,7 +582,7 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 // Four E4M3 bytes as two fp16 pairs.
@@ -622,7 +644,12 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
     const int64_t a = ca + (cz - ca) * warp / W, z = ca + (cz - ca) * (warp + 1) / W;
 
     // launch fields that the loop uses (barrier asm would have them reloaded)
-    const int page = L.page, CK = L.chunk, G = L.G, HB = L.HB, mask_len = static_cast<int>(L.mask_len);
+    const uint32_t page = static_cast<uint32_t>(L.page), page_inv = L.page_inv;
+    auto page_of = [&](int key) {  // key / page: the estimate is at most one too large
+        const uint32_t q = page_inv == 0 ? static_cast<uint32_t>(key) : __umulhi(static_cast<uint32_t>(key), page_inv);
+        return q - (q * page > static_cast<uint32_t>(key) ? 1u : 0u);
+    };
+    const int CK = L.chunk, G = L.G, HB = L.HB, mask_len = static_cast<int>(L.mask_len);
     const int64_t P = L.P, table_ld = L.table_ld;
     const int32_t* table = L.table;
     const void* mask = L.mask.data;
@@ -638,17 +665,23 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
     const bool issues = my_box < C::NBOX;
     int64_t pt = a, prow = 0;
     Unit px{};
-    int plen = 0, pid = -1;
+    int asked = 0, used = 0;  // tiles
+    int plen = 0, pid = -1, pg = 0;
     auto look_up = [&]() {  // unit of tile pt and this lane's page of it
         pid = -1;
-        if (pt >= z) return;
-        if (pt == a || pt == px.t1) {
-            px = unit_at(L, pref, pt);
-            prow = table_row(L, px.b);
-            plen = seq_length(L, px.b);
+        if (pt == px.t1) {
+            const int b = px.b;
+            px = unit_after(L, pref, px);
+            pt = px.t0;
+            if (pt < z && px.b != b) {
+                prow = table_row(L, px.b);
+                plen = seq_length(L, px.b);
+            }
+            pg = px.u / HB;
         }
+        if (pt >= z) return;
         const int key = static_cast<int>(pt - px.t0) * kTile + my_chunk * CK;
-        if (issues && key < plen) pid = table[prow * table_ld + key / page];
+        if (issues && key < plen) pid = table[prow * table_ld + page_of(key)];
     };
     auto request = [&](int slot) {
         const int key = static_cast<int>(pt - px.t0) * kTile + my_chunk * CK;
@@ -666,11 +699,19 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
         __syncwarp();
         if (ok)
             tma_load_4d(ring0 + slot * C::TILE + my_v * C::HALF + my_box * (kTile * RB) + my_chunk * CK * RB,
-                        my_v ? &L.tv : &L.tk, bar, my_box * (RB / EB), key % page, px.u / HB, pid);
+                        my_v ? &L.tv : &L.tk, bar, my_box * (RB / EB), key - static_cast<int>(page_of(key) * page), pg, pid);
         ++pt;
+        ++asked;
         look_up();
     };
-    look_up();
+    if (a < z) {
+        px = unit_at(L, pref, a);
+        pt = px.t0 > a ? px.t0 : a;
+        prow = table_row(L, px.b);
+        plen = seq_length(L, px.b);
+        pg = px.u / HB;
+        look_up();
+    }
     for (int i = 0; i < S && pt < z; ++i) request(i);
 
     // ---- this lane's part of every fragment: keys / elements g and g + 8, heads 2 t and 2 t + 1
@@ -683,22 +724,43 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
     const int v_key = KIND == 2 ? (lane & 15) : ((lane >> 4) * 8 + l7);
     const int v_col = KIND == 2 ? (lane >> 4) : ((lane >> 3) & 1);
 
+    // Scores are in base 2 unless a float mask is added to them (its lowest
+    // values times log2 e would be infinite).
+    const bool biased = mask != nullptr && mask_type != ADA_BOOL;
+    const float unit = biased ? kLog2e : 1.f;
+
     int64_t t = a;
     int slot = 0;             // the ring's slot of tile t and the parity of its barrier
     uint32_t parity = 0;
     bool alive = true;
-    while (t < z && alive) {
-        const Unit x = unit_at(L, pref, t);
+    auto next = [&]() {
+        __syncwarp();  // the slot is read
+        ++used;
+        if (pt < z) request(slot);
+        if (++slot == S) {
+            slot = 0;
+            parity ^= 1u;
+        }
+    };
+    Unit x{-1, 0, z, z};
+    if (a < z) x = unit_at(L, pref, a);
+    int len = 0;
+    for (int len_of = -1; x.t0 < z; x = unit_after(L, pref, x)) {
+        if (t < x.t0) t = x.t0;
         const int64_t tz = x.t1 < z ? x.t1 : z;
         const int g = x.u / HB, h0 = g * G + (x.u % HB) * GB;
         const int heads = min(GB, (g + 1) * G - h0);
-        const int len = seq_length(L, x.b);
+        if (x.b != len_of) {
+            len = seq_length(L, x.b);
+            len_of = x.b;
+        }
+        const float vs = value_scale(L, g);
         const int64_t mrow = x.b * L.mask.s[0], mcol = L.mask.s[1];
         // q^T: element pairs of head fg (of each tile of 8 heads)
         uint32_t qf[D / 16][NT][2];
         float qs[NT][2];
         {
-            const float base = L.scale * (L.k_scale != nullptr ? L.k_scale[g] : 1.f);
+            const float base = L.scale * (L.k_scale != nullptr ? L.k_scale[g] : 1.f) * (biased ? 1.f : kLog2e);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const bool on = n * 8 + fg < heads;
@@ -781,6 +843,10 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
             }
             open = open && ((s_ok[warp * SMAX + slot] >> (lane / CK)) & 1u);
             const uint32_t vis = __ballot_sync(0xffffffffu, open);
+            if (vis == 0u) {  // nothing to see in this tile
+                next();
+                continue;
+            }
             const uint32_t kb = ring0 + slot * C::TILE, vb = kb + C::HALF;
             // S^T = K q^T
             float c[2][NT][4];
@@ -820,12 +886,39 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                     }
             }
             // scores, their maximum over the tile, probabilities
-            float av[2][2];
+            if (vis == 0xffffffffu && !biased) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+                for (int r = 0; r < 2; ++r)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    av[r][j] = mask != nullptr ? __shfl_sync(0xffffffffu, add, r * 16 + j * 8 + fg) : 0.f;
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[r][n][e] *= qs[n][e & 1];
+            } else {
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int key = r * 16 + j * 8 + fg;
+                        const float av = __shfl_sync(0xffffffffu, add, key);
+                        const bool on = (vis >> key) & 1u;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                c[r][n][2 * j + e] = on ? fmaf(c[r][n][2 * j + e], qs[n][e], av) : -INFINITY;
+                    }
+                // a hidden key's values are zeroed, whatever they hold: half a warp per row
+                for (uint32_t hidden = ~vis; hidden != 0; hidden &= hidden - 1) {
+                    const int key = __ffs(hidden) - 1;
+#pragma unroll
+                    for (int x4 = 0; x4 < C::NBOX; ++x4)
+                        if (lane < RB / 4)
+                            *reinterpret_cast<uint32_t*>(ring + slot * C::TILE + C::HALF + x4 * (kTile * RB) + key * RB +
+                                                         lane * 4) = 0u;
+                }
+                fence_proxy_async_smem();  // before the slot's next tile arrives
+                __syncwarp();
+            }
             bool moved = false;
             uint32_t ph[2][NT][2], pl[2][NT][2];
 #pragma unroll
@@ -833,22 +926,14 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                 float ref[2], alpha[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int r = 0; r < 2; ++r)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const float sc = fmaf(c[r][n][2 * j + e], qs[n][e], av[r][j]);
-                            c[r][n][2 * j + e] = ((vis >> (r * 16 + j * 8 + fg)) & 1u) ? sc : -INFINITY;
-                            top = fmaxf(top, c[r][n][2 * j + e]);
-                        }
+                    float top = max3f(max3f(c[0][n][e], c[0][n][2 + e], c[1][n][e]), c[1][n][2 + e], -INFINITY);
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                     const float mn = fmaxf(m[n][e], top);
                     ref[e] = mn == -INFINITY ? 0.f : mn;
                     moved = moved || mn != m[n][e];
-                    alpha[e] = fast_exp2((m[n][e] - ref[e]) * kLog2e);
+                    alpha[e] = fast_exp2((m[n][e] - ref[e]) * unit);
                     m[n][e] = mn;
                     l[n][e] *= alpha[e];
                 }
@@ -856,8 +941,8 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                 for (int r = 0; r < 2; ++r)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float p0 = fast_exp2((c[r][n][2 * j] - ref[0]) * kLog2e);
-                        const float p1 = fast_exp2((c[r][n][2 * j + 1] - ref[1]) * kLog2e);
+                        const float p0 = fast_exp2((c[r][n][2 * j] - ref[0]) * unit);
+                        const float p1 = fast_exp2((c[r][n][2 * j + 1] - ref[1]) * unit);
                         l[n][0] += p0;
                         l[n][1] += p1;
                         uint32_t hi, lo;
@@ -876,20 +961,10 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                 }
                 moved = false;
             }
-            // O^T += V^T P^T; a hidden key's values are zeroed, whatever they hold
+            // O^T += V^T P^T
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const uint32_t seen = (vis >> (r * 16)) & 0xFFFFu;
-                const uint32_t pair0 = (seen >> (2 * ft)) & 3u, pair1 = (seen >> (2 * ft + 8)) & 3u;
-                const uint32_t keep0 = (pair0 & 1u ? 0xFFFFu : 0u) | (pair0 & 2u ? 0xFFFF0000u : 0u);
-                const uint32_t keep1 = (pair1 & 1u ? 0xFFFFu : 0u) | (pair1 & 2u ? 0xFFFF0000u : 0u);
                 auto product = [&](int i, uint32_t (&f)[4]) {
-                    if (seen != 0xFFFFu) {
-                        f[0] &= keep0;
-                        f[1] &= keep0;
-                        f[2] &= keep1;
-                        f[3] &= keep1;
-                    }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         mma_16816<KIND>(o[i][n], f, ph[r][n][0], ph[r][n][1]);
@@ -920,18 +995,12 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                     }
                 }
             }
-            __syncwarp();  // the slot is read
-            if (pt < z) request(slot);
-            if (++slot == S) {
-                slot = 0;
-                parity ^= 1u;
-            }
+            next();
         }
         if (!alive) break;
         const bool whole = x.t0 >= a && x.t1 <= z;
         const int side = x.t0 < a ? 0 : 1, left = warp * 2 + side;
         float* part = J.part(warp, side);
-        const float vs = value_scale(L, g);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -943,6 +1012,7 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                 const int h = n * 8 + 2 * ft + e;
                 if (h >= heads) continue;
                 const float inv = whole ? (sum == 0.f ? 0.f : vs / sum) : 1.f;
+                const float mn = biased ? m[n][e] : m[n][e] * kLn2;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -954,9 +1024,9 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                     }
                 if (fg == 0) {
                     if (whole) {
-                        if (L.lse != nullptr) L.lse[static_cast<int64_t>(x.b) * L.H + h0 + h] = m[n][e] + logf(sum);
+                        if (L.lse != nullptr) L.lse[static_cast<int64_t>(x.b) * L.H + h0 + h] = mn + logf(sum);
                     } else {
-                        J.ml[(left * GB + h) * 2] = m[n][e];
+                        J.ml[(left * GB + h) * 2] = mn;
                         J.ml[(left * GB + h) * 2 + 1] = sum;
                     }
                 }
@@ -965,7 +1035,7 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
         __syncwarp();
     }
     if (!alive) {  // a wait ran out (recorded): the tiles still requested are awaited, then the block gives up
-        for (; t < pt; ++t) {
+        for (; asked > used; ++used) {
             const uint64_t t0 = globaltimer_ns();
             while (!mbar_try_wait(bar0 + slot * 8, parity) && globaltimer_ns() - t0 < limit) {}
             if (++slot == S) {
