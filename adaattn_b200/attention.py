@@ -256,6 +256,49 @@ class AdaAttention(nn.Module):
         except torch.cuda.OutOfMemoryError as e:
             raise MemoryError(f"GPU out of memory: {e}") from e
 
+    def forward_cached(self, x: Tensor, cache, layer: int, *, seqs: Optional[Tensor] = None,
+                       new_tokens: Optional[Tensor] = None, residual: Optional[Tensor] = None) -> Tensor:
+        """Self-attention of the newest tokens with a ``PagedKVCache``: x
+        [B, N, E] -> [B, N, E] (plus ``residual`` when given), their keys and
+        values appended to the cache's layer. The cache must have reserved
+        them (``cache.reserve``) for the table rows ``seqs`` (int32; row b for
+        b when omitted).
+
+        N = 1: each token attends to its sequence's whole cache
+        (``paged_attention``). N > 1: the prompts of sequences that hold
+        nothing else, right-padded to N with new_tokens[b] real tokens each
+        (N when omitted), run through the causal attention of ``forward``.
+        Heads are dense: the module must be causal and built with
+        ``enable_adaptive_rank=False``, since a low-rank decision taken for a
+        prompt has no counterpart over the cache. Inference only (eval mode,
+        no autograd); the statistics count the prompts.
+        """
+        if not self.causal:
+            raise RuntimeError("cached decoding needs a causal module (causal=True)")
+        if self.enable_adaptive_rank:
+            raise RuntimeError("cached decoding computes dense heads; build the module with "
+                               "enable_adaptive_rank=False")
+        if self.training and (self.attn_dropout.p > 0 or self.resid_dropout.p > 0):
+            raise RuntimeError("cached decoding is for inference: call eval()")
+        if x.ndim != 3 or x.shape[-1] != self.embed_dim:
+            raise ShapeError("x must be [B, N, E]", expected_shape=(None, None, self.embed_dim),
+                             actual_shape=tuple(x.shape))
+        b, n, e = x.shape
+        h, d = self.num_heads, self.head_dim
+        with torch.no_grad():
+            w, bias = self._stacked_qkv()
+            qkv = (core.linear(x, w, bias) if self._dense_on_tensor_cores(x)
+                   else torch.nn.functional.linear(x, w, bias))
+            q, k, v = (qkv[..., i * e:(i + 1) * e].view(b, n, h, d).transpose(1, 2) for i in range(3))
+            cache.append(layer, k, v, new_tokens, seqs=seqs)
+            if n == 1:
+                merged = cache.attend(layer, q[:, :, 0], seqs=seqs, scale=self.scale).view(b, 1, e)
+            else:
+                merged = torch.empty(b, n, h, d, dtype=q.dtype, device=q.device)
+                self.attention_core(q, k, v, out=merged.transpose(1, 2))
+                merged = merged.view(b, n, e)
+            return self._linear(self.out_proj, merged, residual)
+
     @staticmethod
     def _dense_on_tensor_cores(x: Tensor) -> bool:
         # The tensor-core layer (core.linear) serves 16-bit CUDA tensors; fp32

@@ -28,7 +28,7 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;       // keys per tile
-constexpr int kLead = 3;        // places before a unit's tiles
+constexpr int kLead = 6;        // places before a unit's tiles (3: the ragged 8-bit batch took 205 us, 6: 197)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -551,9 +551,7 @@ struct TcCfg {
     static constexpr int NBOX = D * EB / RB;
     static constexpr int HALF = kTile * D * EB;              // K or V bytes of a tile
     static constexpr int TILE = 2 * HALF;
-    // 8-bit pages of 128 elements are bound by the instructions between their
-    // bytes, which more warps overlap: 10 of 2 stages instead of 8 of 3.
-    static constexpr int WARPS = TILE >= 16384 ? 4 : (KIND == 2 && D == 128 && NT == 1) ? 10 : 8;
+    static constexpr int WARPS = TILE >= 16384 ? 4 : 8;      // (10 with 2 stages for 8-bit pages: 3 % slower)
     static constexpr int STAGES = TILE >= 8192 ? 3 : 6;      // at most; fewer when the rest needs the space
     static constexpr int GB = 8 * NT;
     static constexpr int PART = GB * D;                      // floats a warp leaves per slot

@@ -5,16 +5,22 @@ examples/transformer_integration.py:12-141 (post-LayerNorm blocks, GELU
 feed-forward, learned positions, head tied to the token embedding,
 non-causal attention), with this package's AdaAttention inside. Used to
 measure the module-level throughput of the path; the model itself is not part
-of the hot path.
+of the hot path. Built causal and dense (``causal=True,
+enable_adaptive_rank=False``) it also decodes token by token over a paged
+cache and scores given tokens.
 """
 
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 import torch.nn as nn
 
 from . import core
 from .attention import AdaAttention
+from .paged import PagedKVCache
+from .scoring import TokenLogprobs, token_logprobs
 
 
 def _norm(norm: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
@@ -52,6 +58,17 @@ class TransformerBlock(nn.Module):
             return _norm(self.norm2, core.linear(f, down.weight, down.bias, residual=x))
         attn_out, _ = self.attention(x, x, x, attention_mask=attention_mask)
         x = self.norm1(x + attn_out)
+        return self.norm2(x + self.ff(x))
+
+    def forward_cached(self, x: torch.Tensor, cache, layer: int, **kwargs) -> torch.Tensor:
+        """The block on the newest tokens, with the layer's ``PagedKVCache``
+        (``AdaAttention.forward_cached``)."""
+        if self._fused(x):
+            x = _norm(self.norm1, self.attention.forward_cached(x, cache, layer, residual=x, **kwargs))
+            up, down = self.ff[0], self.ff[3]
+            f = core.linear(x, up.weight, up.bias, activation="gelu")
+            return _norm(self.norm2, core.linear(f, down.weight, down.bias, residual=x))
+        x = self.norm1(x + self.attention.forward_cached(x, cache, layer, **kwargs))
         return self.norm2(x + self.ff(x))
 
     def _fused(self, x: torch.Tensor) -> bool:
@@ -101,6 +118,60 @@ class AdaptiveTransformer(nn.Module):
         for block in self.blocks:
             x = block(x, attention_mask=attention_mask)
         return self._logits(_norm(self.norm, x))
+
+    # -- serving: a paged cache, one token at a time, scores of given tokens --------
+    def make_cache(self, num_pages: int, page_size: int, *, max_sequences: int, dtype=None, **kwargs) -> PagedKVCache:
+        """A ``PagedKVCache`` for this decoder's layers and heads, in the
+        weights' dtype unless given another (float8_e4m3fn for 8 bits)."""
+        attn = self.blocks[0].attention
+        weight = attn.q_proj.weight
+        return PagedKVCache(len(self.blocks), num_pages, page_size, attn.num_heads, attn.head_dim,
+                            max_sequences=max_sequences,
+                            max_pages_per_sequence=-(-self.max_seq_len // page_size),
+                            dtype=weight.dtype if dtype is None else dtype, device=weight.device, **kwargs)
+
+    @torch.no_grad()
+    def prefill(self, input_ids: torch.Tensor, cache: PagedKVCache, seqs: torch.Tensor,
+                lengths: Optional[torch.Tensor] = None):
+        """Starts sequences: the table rows ``seqs`` (int32 [B]) give up what
+        they held and take the prompts input_ids [B, N], right-padded, of
+        ``lengths`` (int32 [B]; N when omitted, at least 1). Returns (logits of each
+        prompt's last token [B, V], the tokens the cache granted; 0 for a
+        sequence that found no free pages, whose logits mean nothing)."""
+        b, n = input_ids.shape
+        if lengths is None:
+            lengths = torch.full((b,), n, dtype=torch.int32, device=input_ids.device)
+        cache.free(seqs)
+        granted = cache.reserve(seqs, lengths)
+        pos = torch.arange(n, device=input_ids.device).unsqueeze(0)
+        x = self._cached_layers(self.token_embedding(input_ids) + self.position_embedding(pos), cache, seqs, granted)
+        last = (lengths.long() - 1).clamp(0, n - 1)
+        return self._logits(_norm(self.norm, x[torch.arange(b, device=x.device), last])), granted
+
+    @torch.no_grad()
+    def decode_step(self, input_ids: torch.Tensor, cache: PagedKVCache, seqs: torch.Tensor):
+        """One more token input_ids [B] of each sequence: (logits of the next
+        one [B, V], the tokens granted, 1 or 0). Nothing waits for the host, so
+        a step can be captured in a CUDA graph and replayed."""
+        ones = torch.ones_like(seqs)
+        granted = cache.reserve(seqs, ones)
+        # a sequence that was refused keeps its last position (its logits mean nothing)
+        pos = (cache.seq_lens[seqs.long()].long() - 1).clamp(0, self.max_seq_len - 1)
+        x = (self.token_embedding(input_ids) + self.position_embedding(pos)).unsqueeze(1)
+        x = self._cached_layers(x, cache, seqs, granted)
+        return self._logits(_norm(self.norm, x))[:, 0], granted
+
+    def _cached_layers(self, x, cache, seqs, granted):
+        for i, block in enumerate(self.blocks):
+            x = block.forward_cached(x, cache, i, seqs=seqs, new_tokens=granted)
+        return x
+
+    def score(self, input_ids: torch.Tensor, *, top_k: int = 0, attention_mask=None) -> TokenLogprobs:
+        """Log probability of each token of input_ids [B, N] after the first
+        given those before it ([B, N - 1]), with entropies and top_k
+        alternatives (``token_logprobs``); differentiable. For a causal decoder."""
+        logits = self.forward(input_ids, attention_mask=attention_mask)
+        return token_logprobs(logits[:, :-1], input_ids[:, 1:], top_k=top_k)
 
     def _logits(self, h: torch.Tensor) -> torch.Tensor:
         """The tied head. A vocabulary that is not a multiple of 64 (50257)
