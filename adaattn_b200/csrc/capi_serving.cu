@@ -195,7 +195,10 @@ int pages_table(const AdaTensor* table, const AdaTensor* lens, const AdaTensor* 
     if ((rc = check_table(table, lens)) || (rc = check_ints(refs, "ref_counts", -1))) return rc;
     if (page < 1 || page > 65536) return fail(ADA_ERR_UNSUPPORTED, "page size %lld outside [1, 65536]", (long long)page);
     if ((rc = check_width(table, page))) return rc;
-    if (refs->shape[0] > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "at most 2^31 - 1 pages");
+    if (refs->shape[0] > (int64_t(1) << 30)) return fail(ADA_ERR_UNSUPPORTED, "at most 2^30 pages");
+    // the pages that a call can need are counted in 32 bits
+    if (table->shape[0] * (table->shape[1] + 1) > kMaxInt)
+        return fail(ADA_ERR_UNSUPPORTED, "page_table has 2^31 or more entries");
     if (table->shape[0] > 1 && table->stride[0] < table->shape[1])
         return fail(ADA_ERR_LAYOUT, "the rows of page_table overlap");
     *L = PagesLaunch{};
@@ -224,6 +227,10 @@ int pages_data(const AdaTensor* pages, void* workspace, size_t bytes, PagesLaunc
     L->plane_bytes = row_stride(pages, 0) * eb;
     if (pages->shape[1] > 1 && pages->stride[1] < pages->shape[2]) return fail(ADA_ERR_LAYOUT, "pages overlap");
     if (pages->shape[0] > 1 && pages->stride[0] < pages->shape[2]) return fail(ADA_ERR_LAYOUT, "planes overlap");
+    if (pages->shape[0] > 1 && pages->shape[1] > 1) {  // one of the two lies inside the other's stride
+        const int in = pages->stride[0] < pages->stride[1] ? 0 : 1;
+        if (pages->stride[1 - in] < pages->stride[in] * pages->shape[in]) return fail(ADA_ERR_LAYOUT, "pages and planes overlap");
+    }
     const uint64_t all = reinterpret_cast<uint64_t>(pages->data) | static_cast<uint64_t>(L->page_bytes) |
                          static_cast<uint64_t>(L->page_stride) | static_cast<uint64_t>(L->plane_bytes);
     L->vec = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;

@@ -19,6 +19,7 @@ import torch.nn as nn
 
 from . import core
 from .attention import AdaAttention
+from .config import ShapeError
 from .paged import PagedKVCache
 from .scoring import TokenLogprobs, token_logprobs
 
@@ -139,8 +140,11 @@ class AdaptiveTransformer(nn.Module):
         prompt's last token [B, V], the tokens the cache granted; 0 for a
         sequence that found no free pages, whose logits mean nothing)."""
         b, n = input_ids.shape
+        if n < 1 or n > self.max_seq_len:
+            raise ShapeError(f"prompts hold 1 to {self.max_seq_len} tokens, got {n}")
         if lengths is None:
             lengths = torch.full((b,), n, dtype=torch.int32, device=input_ids.device)
+        lengths = lengths.clamp(0, n)
         cache.free(seqs)
         granted = cache.reserve(seqs, lengths)
         pos = torch.arange(n, device=input_ids.device).unsqueeze(0)
@@ -151,12 +155,12 @@ class AdaptiveTransformer(nn.Module):
     @torch.no_grad()
     def decode_step(self, input_ids: torch.Tensor, cache: PagedKVCache, seqs: torch.Tensor):
         """One more token input_ids [B] of each sequence: (logits of the next
-        one [B, V], the tokens granted, 1 or 0). Nothing waits for the host, so
-        a step can be captured in a CUDA graph and replayed."""
-        ones = torch.ones_like(seqs)
-        granted = cache.reserve(seqs, ones)
-        # a sequence that was refused keeps its last position (its logits mean nothing)
-        pos = (cache.seq_lens[seqs.long()].long() - 1).clamp(0, self.max_seq_len - 1)
+        one [B, V], the tokens granted: 1, or 0 for a sequence that found no
+        free page or is max_seq_len long, whose logits mean nothing). Nothing
+        waits for the host, so a step can be captured in a CUDA graph and replayed."""
+        rows = seqs.long().clamp(0, cache.seq_lens.shape[0] - 1)
+        granted = cache.reserve(seqs, (cache.seq_lens[rows] < self.max_seq_len).to(torch.int32))
+        pos = (cache.seq_lens[rows].long() - 1).clamp(0, self.max_seq_len - 1)
         x = (self.token_embedding(input_ids) + self.position_embedding(pos)).unsqueeze(1)
         x = self._cached_layers(x, cache, seqs, granted)
         return self._logits(_norm(self.norm, x))[:, 0], granted

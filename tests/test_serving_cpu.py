@@ -121,6 +121,11 @@ def test_page_operations_refuse_before_any_device_work():
     assert lib.ada_pages_compact(p, *pool, 16, T(two), None, 0, None) == SHAPE
     assert lib.ada_pages_compact(_planes(data.expand(2, 7, 2, 16, 8)[:1].expand(2, 7, 2, 16, 8)), *pool, 16, T(one),
                                  None, 0, None) == LAYOUT
+    both = torch.zeros(14 * 256)  # planes and pages a page apart: they overlap
+    assert lib.ada_pages_compact(_planes(both.as_strided((2, 7, 2, 16, 8), (256, 256, 128, 8, 1))), *pool, 16, T(one),
+                                 None, 0, None) == LAYOUT
+    wide = torch.zeros(1, dtype=i32).expand(2 ** 16, 1).as_strided((2 ** 16, 2 ** 15), (0, 0))
+    assert lib.ada_pages_free(T(wide), T(torch.zeros(2 ** 16, dtype=i32)), T(refs), 16, T(one), None) in (LAYOUT, UNSUPPORTED)
     with pytest.raises(ada.ShapeError):
         _planes(data.transpose(3, 4))
 

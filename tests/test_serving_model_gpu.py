@@ -164,6 +164,26 @@ def test_a_pool_that_runs_out(cuda_device):
     _lib.poll_device_status(dev)
 
 
+def test_sequences_end_at_the_models_length(cuda_device):
+    """max_seq_len 96 in pages of 20: the fifth page has room for four more tokens than the model has positions."""
+    dev = cuda_device
+    m = _model(dev, torch.bfloat16)
+    ids = torch.randint(0, V, (2, 96), generator=torch.Generator().manual_seed(7)).to(dev)
+    cache = m.make_cache(12, 20, max_sequences=3)
+    _, granted = m.prefill(ids[:, :95], cache, _ids([0, 2], dev), _ids([95, 200], dev))
+    assert granted.tolist() == [95, 95]
+    seqs = _ids([0, 2], dev)
+    assert m.decode_step(ids[:, 95], cache, seqs)[1].tolist() == [1, 1]
+    assert m.decode_step(ids[:, 95], cache, seqs)[1].tolist() == [0, 0]
+    assert cache.seq_lens.tolist() == [96, 0, 96]
+    _lib.poll_device_status(dev)
+    assert m.decode_step(ids[:, 0], cache, _ids([1, 9], dev))[1].tolist() == [1, 0]  # row 9 does not exist
+    with pytest.raises(ada.KernelError):
+        _lib.poll_device_status(dev)
+    with pytest.raises(ada.ShapeError):
+        m.prefill(torch.zeros(1, 97, dtype=torch.int64, device=dev), cache, _ids([0], dev))
+
+
 def test_score_and_its_gradient(cuda_device):
     """score() against log_softmax of the same logits; its gradient reaches the
     weights like that of the plain formula, to the roundings of the bf16 logits' gradient."""
