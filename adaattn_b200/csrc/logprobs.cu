@@ -18,7 +18,10 @@
 // at 6.5 TB/s an SM takes 11.7 16-bit elements a cycle, of 128 instruction
 // lanes and 16 exponentials. Unpacking (1), clamping and the maximum on packed
 // pairs (1/2 each), argument, sum and weighted sum as packed fp32 pairs (1/2
-// each) and the exponential make 4.5. Logits are clamped from below (-2^100;
+// each) and the exponential make 4.5; with moves, addresses and each row's end
+// the counters show 10.8, and 16384 rows of 50257 bf16 logits take 300 us (5.5
+// TB/s; fp32 473 us, 7.0 TB/s), 385 us with 5 and 437 us with 20 alternatives.
+// The gradient runs at 6.5 TB/s of reads and writes. Logits are clamped from below (-2^100;
 // fp16: its lowest value) so that -inf stays out of the weighted sum; a row
 // with nothing above the clamp is done again by the plain formulas.
 //
