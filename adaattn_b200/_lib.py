@@ -59,6 +59,7 @@ class AdaFwdParams(Structure):
 
 
 _T = POINTER(AdaTensor)
+_P = c_char_p  # an AdaTensor's bytes (``packed``)
 _SIGNATURES = {
     "ada_abi_version": (c_int32, []),
     "ada_get_last_error": (c_int32, [c_char_p, c_size_t]),
@@ -88,19 +89,19 @@ _SIGNATURES = {
     "ada_layer_norm": (c_int32, [_T, _T, _T, c_float, _T, c_void_p]),
     "ada_record_statistics": (c_int32, [c_void_p, _T, _T, _T, c_void_p]),
     "ada_paged_attn_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
-    "ada_paged_attn": (c_int32, [_T, _T, _T, _T, _T, _T, _T, _T, _T, c_float, _T, c_void_p, c_void_p,
+    "ada_paged_attn": (c_int32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_float, _P, c_void_p, c_void_p,
                                  c_size_t, c_void_p]),
-    "ada_paged_append": (c_int32, [_T, _T, _T, _T, _T, _T, _T, _T, _T, _T, c_void_p]),
+    "ada_paged_append": (c_int32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_void_p]),
     "ada_pages_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
-    "ada_pages_free": (c_int32, [_T, _T, _T, c_int64, _T, c_void_p]),
-    "ada_pages_fork": (c_int32, [_T, _T, _T, c_int64, _T, _T, c_void_p]),
-    "ada_pages_reserve": (c_int32, [_T, _T, _T, _T, c_int64, _T, _T, _T, c_void_p, c_size_t, c_void_p]),
-    "ada_pages_copy": (c_int32, [_T, _T, _T, _T, c_int64, _T, _T, _T, c_void_p, c_size_t, c_void_p]),
-    "ada_pages_compact": (c_int32, [_T, _T, _T, _T, c_int64, _T, c_void_p, c_size_t, c_void_p]),
-    "ada_token_logprobs": (c_int32, [_T, _T, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
+    "ada_pages_free": (c_int32, [_P, _P, _P, c_int64, _P, c_void_p]),
+    "ada_pages_fork": (c_int32, [_P, _P, _P, c_int64, _P, _P, c_void_p]),
+    "ada_pages_reserve": (c_int32, [_P, _P, _P, _P, c_int64, _P, _P, _P, c_void_p, c_size_t, c_void_p]),
+    "ada_pages_copy": (c_int32, [_P, _P, _P, _P, c_int64, _P, _P, _P, c_void_p, c_size_t, c_void_p]),
+    "ada_pages_compact": (c_int32, [_P, _P, _P, _P, c_int64, _P, c_void_p, c_size_t, c_void_p]),
+    "ada_token_logprobs": (c_int32, [_P, _P, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_void_p]),
-    "ada_token_logprobs_bwd": (c_int32, [_T, _T, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
-                                         c_void_p, _T, c_void_p]),
+    "ada_token_logprobs_bwd": (c_int32, [_P, _P, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                         c_void_p, _P, c_void_p]),
     "ada_rsvd_workspace_bytes": (c_size_t, [_T, _T, c_int32]),
     "ada_rsvd": (c_int32, [_T, _T, c_int32, c_int32, _T, _T, _T, c_void_p, c_size_t, c_void_p]),
 }
@@ -161,6 +162,12 @@ _PAD = ((0, 0, 0, 0), (0, 0, 0), (0, 0), (0,), ())
 
 def tensor(t: torch.Tensor) -> AdaTensor:
     """Describe a torch tensor (up to 4-D) for the C ABI; no copy."""
+    return AdaTensor.from_buffer_copy(packed(t))
+
+
+def packed(t: torch.Tensor) -> bytes:
+    """``tensor``'s bytes, which the entry points declared with ``_P`` take as
+    they are (an AdaTensor pointer to the bytes' own storage)."""
     shape = t.shape
     nd = len(shape)
     if nd > 4:
@@ -169,8 +176,7 @@ def tensor(t: torch.Tensor) -> AdaTensor:
     if code is None:
         raise TypeError(f"unsupported dtype {t.dtype}")
     pad = _PAD[nd]
-    return AdaTensor.from_buffer_copy(
-        _pack_tensor(0 if 0 in shape else t.data_ptr(), code, nd, *shape, *pad, *t.stride(), *pad))
+    return _pack_tensor(0 if 0 in shape else t.data_ptr(), code, nd, *shape, *pad, *t.stride(), *pad)
 
 
 def stream_ptr(device: torch.device) -> int:

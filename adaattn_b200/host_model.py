@@ -20,7 +20,7 @@ import torch.nn as nn
 from . import core
 from .attention import AdaAttention
 from .config import ShapeError
-from .paged import PagedKVCache
+from .paged import PagedKVCache, _ids
 from .scoring import TokenLogprobs, token_logprobs
 
 
@@ -144,7 +144,7 @@ class AdaptiveTransformer(nn.Module):
             raise ShapeError(f"prompts hold 1 to {self.max_seq_len} tokens, got {n}")
         if lengths is None:
             lengths = torch.full((b,), n, dtype=torch.int32, device=input_ids.device)
-        lengths = lengths.clamp(0, n)
+        lengths, seqs = lengths.clamp(0, n), _ids(seqs, cache.device)
         cache.free(seqs)
         granted = cache.reserve(seqs, lengths)
         pos = torch.arange(n, device=input_ids.device).unsqueeze(0)
@@ -157,7 +157,9 @@ class AdaptiveTransformer(nn.Module):
         """One more token input_ids [B] of each sequence: (logits of the next
         one [B, V], the tokens granted: 1, or 0 for a sequence that found no
         free page or is max_seq_len long, whose logits mean nothing). Nothing
-        waits for the host, so a step can be captured in a CUDA graph and replayed."""
+        waits for the host, so a step can be captured in a CUDA graph (after a
+        first eager one, which stacks the weights) and replayed."""
+        seqs = _ids(seqs, cache.device)
         rows = seqs.long().clamp(0, cache.seq_lens.shape[0] - 1)
         granted = cache.reserve(seqs, (cache.seq_lens[rows] < self.max_seq_len).to(torch.int32))
         pos = (cache.seq_lens[rows].long() - 1).clamp(0, self.max_seq_len - 1)

@@ -39,14 +39,14 @@ Ids = Union[torch.Tensor, Sequence[int]]
 
 
 def _device_of(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> torch.device:
-    dev = first.device
-    if not first.is_cuda:
-        raise RuntimeError(f"adaattn_b200 runs on CUDA devices only (sm_100a); got a tensor on {dev}. "
+    index = first.get_device()
+    if index < 0:
+        raise RuntimeError(f"adaattn_b200 runs on CUDA devices only (sm_100a); got a tensor on {first.device}. "
                            "There is no CPU path.")
     for t in rest:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"all tensors must be on {dev}; got one on {t.device}")
-    return dev
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"all tensors must be on {first.device}; got one on {t.device}")
+    return first.device
 
 
 def _no_grad(what: str, *ts: Optional[torch.Tensor]) -> None:
@@ -55,7 +55,7 @@ def _no_grad(what: str, *ts: Optional[torch.Tensor]) -> None:
 
 
 def _opt(t: Optional[torch.Tensor]):
-    return None if t is None else _lib.tensor(t)
+    return None if t is None else _lib.packed(t)
 
 
 def _call(what: str, dev: torch.device, fn, *args) -> None:
@@ -118,9 +118,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         key_mask = key_mask.float()
     lib = _lib.load()
     ws = torch.empty(_attn_workspace(b, h, max(1, k_pages.shape[1]), d), dtype=torch.uint8, device=dev)
-    _call("ada_paged_attn", dev, lib.ada_paged_attn, _lib.tensor(_unit_last(q)), _lib.tensor(k_pages),
-          _lib.tensor(v_pages), _lib.tensor(page_table), _lib.tensor(seq_lens), _opt(seqs), _opt(key_mask),
-          _opt(k_scale), _opt(v_scale), float(d ** -0.5 if scale is None else scale), _lib.tensor(out),
+    _call("ada_paged_attn", dev, lib.ada_paged_attn, _lib.packed(_unit_last(q)), _lib.packed(k_pages),
+          _lib.packed(v_pages), _lib.packed(page_table), _lib.packed(seq_lens), _opt(seqs), _opt(key_mask),
+          _opt(k_scale), _opt(v_scale), float(d ** -0.5 if scale is None else scale), _lib.packed(out),
           None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel())
     return out if lse is None else (out, lse)
 
@@ -141,12 +141,12 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     """
     dev = _device_of(k, v, k_pages, v_pages, page_table, seq_lens, new_tokens, seqs, k_scale, v_scale)
     _no_grad("paged_append", k, v, k_pages, v_pages)
-    _call("ada_paged_append", dev, _lib.load().ada_paged_append, _lib.tensor(_unit_last(k)),
-          _lib.tensor(_unit_last(v)), _lib.tensor(k_pages), _lib.tensor(v_pages), _lib.tensor(page_table),
-          _lib.tensor(seq_lens), _opt(new_tokens), _opt(seqs), _opt(k_scale), _opt(v_scale))
+    _call("ada_paged_append", dev, _lib.load().ada_paged_append, _lib.packed(_unit_last(k)),
+          _lib.packed(_unit_last(v)), _lib.packed(k_pages), _lib.packed(v_pages), _lib.packed(page_table),
+          _lib.packed(seq_lens), _opt(new_tokens), _opt(seqs), _opt(k_scale), _opt(v_scale))
 
 
-def _planes(pages: torch.Tensor) -> _lib.AdaTensor:
+def _planes(pages: torch.Tensor) -> bytes:
     """[planes, P, ...] as [planes, P, elements of a page] (page blocks must be contiguous)."""
     if pages.dim() < 3:
         raise ShapeError(f"pages must be [planes, P, ...], got {pages.dim()}-D")
@@ -156,7 +156,7 @@ def _planes(pages: torch.Tensor) -> _lib.AdaTensor:
         if shape[i] > 1 and stride[i] != inner:
             raise ShapeError("the pages' blocks must be contiguous")
         inner *= shape[i]
-    return _lib.tensor(pages.as_strided((shape[0], shape[1], inner), (stride[0], stride[1], 1)))
+    return _lib.packed(pages.as_strided((shape[0], shape[1], inner), (stride[0], stride[1], 1)))
 
 
 def _page_size(pages: torch.Tensor, page_size: Optional[int]) -> int:
@@ -187,9 +187,9 @@ def reserve_pages(pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch
     dev = _device_of(pages, page_table, seq_lens, ref_counts, seqs, new_tokens)
     granted = torch.empty(seqs.shape, dtype=torch.int32, device=dev)
     ws = _workspace(page_table, ref_counts, seqs.numel())
-    _call("ada_pages_reserve", dev, _lib.load().ada_pages_reserve, _planes(pages), _lib.tensor(page_table),
-          _lib.tensor(seq_lens), _lib.tensor(ref_counts), _page_size(pages, page_size), _lib.tensor(seqs),
-          _lib.tensor(new_tokens), _lib.tensor(granted), ws.data_ptr(), ws.numel())
+    _call("ada_pages_reserve", dev, _lib.load().ada_pages_reserve, _planes(pages), _lib.packed(page_table),
+          _lib.packed(seq_lens), _lib.packed(ref_counts), _page_size(pages, page_size), _lib.packed(seqs),
+          _lib.packed(new_tokens), _lib.packed(granted), ws.data_ptr(), ws.numel())
     return granted
 
 
@@ -199,8 +199,8 @@ def fork_pages(page_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: tor
     (``ada_pages_fork``); no data moves. A dst named twice counts once, one
     that is also a src of the call is left out."""
     dev = _device_of(page_table, seq_lens, ref_counts, src, dst)
-    _call("ada_pages_fork", dev, _lib.load().ada_pages_fork, _lib.tensor(page_table), _lib.tensor(seq_lens),
-          _lib.tensor(ref_counts), int(page_size), _lib.tensor(src), _lib.tensor(dst))
+    _call("ada_pages_fork", dev, _lib.load().ada_pages_fork, _lib.packed(page_table), _lib.packed(seq_lens),
+          _lib.packed(ref_counts), int(page_size), _lib.packed(src), _lib.packed(dst))
 
 
 def copy_pages(pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -212,9 +212,9 @@ def copy_pages(pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Te
     dev = _device_of(pages, page_table, seq_lens, ref_counts, src, dst)
     granted = torch.empty(src.shape, dtype=torch.int32, device=dev)
     ws = _workspace(page_table, ref_counts, src.numel())
-    _call("ada_pages_copy", dev, _lib.load().ada_pages_copy, _planes(pages), _lib.tensor(page_table),
-          _lib.tensor(seq_lens), _lib.tensor(ref_counts), _page_size(pages, page_size), _lib.tensor(src),
-          _lib.tensor(dst), _lib.tensor(granted), ws.data_ptr(), ws.numel())
+    _call("ada_pages_copy", dev, _lib.load().ada_pages_copy, _planes(pages), _lib.packed(page_table),
+          _lib.packed(seq_lens), _lib.packed(ref_counts), _page_size(pages, page_size), _lib.packed(src),
+          _lib.packed(dst), _lib.packed(granted), ws.data_ptr(), ws.numel())
     return granted
 
 
@@ -223,8 +223,8 @@ def free_pages(page_table: torch.Tensor, seq_lens: torch.Tensor, ref_counts: tor
     """The sequences give their pages up: length 0, table entries -1
     (``ada_pages_free``). A sequence named twice is freed once."""
     dev = _device_of(page_table, seq_lens, ref_counts, seqs)
-    _call("ada_pages_free", dev, _lib.load().ada_pages_free, _lib.tensor(page_table), _lib.tensor(seq_lens),
-          _lib.tensor(ref_counts), int(page_size), _lib.tensor(seqs))
+    _call("ada_pages_free", dev, _lib.load().ada_pages_free, _lib.packed(page_table), _lib.packed(seq_lens),
+          _lib.packed(ref_counts), int(page_size), _lib.packed(seqs))
 
 
 def compact_pages(pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -235,8 +235,8 @@ def compact_pages(pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch
     dev = _device_of(pages, page_table, seq_lens, ref_counts)
     live = torch.empty(1, dtype=torch.int32, device=dev)
     ws = _workspace(page_table, ref_counts, 0)
-    _call("ada_pages_compact", dev, _lib.load().ada_pages_compact, _planes(pages), _lib.tensor(page_table),
-          _lib.tensor(seq_lens), _lib.tensor(ref_counts), _page_size(pages, page_size), _lib.tensor(live),
+    _call("ada_pages_compact", dev, _lib.load().ada_pages_compact, _planes(pages), _lib.packed(page_table),
+          _lib.packed(seq_lens), _lib.packed(ref_counts), _page_size(pages, page_size), _lib.packed(live),
           ws.data_ptr(), ws.numel())
     return live
 

@@ -53,14 +53,18 @@ def _grad_like(z3: torch.Tensor) -> torch.Tensor:
     return torch.empty(a, r, ld, dtype=z3.dtype, device=z3.device)[..., :v]
 
 
-def _forward(z3: torch.Tensor, tokens: torch.Tensor, top_k: int, ignore_index: int):
+def _forward(z3: torch.Tensor, tokens: torch.Tensor, top_k: int, ignore_index: int, views: bool = True):
+    """``views``: the three vectors and the statistics may share one buffer."""
     dev = z3.device
     rows = z3.shape[0] * z3.shape[1]
-    lp, ent, lse = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(3))
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
+    if views:
+        lp, ent, lse, stats, _ = torch.empty(5, rows, dtype=torch.float32, device=dev).unbind(0)
+    else:
+        lp, ent, lse = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(3))
+        stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
     top_lp = torch.empty(rows, top_k, dtype=torch.float32, device=dev) if top_k else None
     top_id = torch.empty(rows, top_k, dtype=torch.int64, device=dev) if top_k else None
-    _call("ada_token_logprobs", dev, _lib.load().ada_token_logprobs, _lib.tensor(z3), _lib.tensor(tokens),
+    _call("ada_token_logprobs", dev, _lib.load().ada_token_logprobs, _lib.packed(z3), _lib.packed(tokens),
           int(ignore_index), int(top_k), lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), stats.data_ptr(),
           _lib.ptr(top_lp), _lib.ptr(top_id))
     return lp, ent, lse, top_lp, top_id, stats
@@ -78,9 +82,9 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, stats: t
     ups = [None if g is None else g.float().contiguous() for g in (grad_logprobs, grad_entropy, grad_lse)]
     dev = _device_of(logits, tokens, stats, entropy, *ups)
     grad = _grad_like(logits)
-    _call("ada_token_logprobs_bwd", dev, _lib.load().ada_token_logprobs_bwd, _lib.tensor(logits),
-          _lib.tensor(tokens), int(ignore_index), stats.data_ptr(), entropy.data_ptr(),
-          *(_lib.ptr(g) or None for g in ups), _lib.tensor(grad))
+    _call("ada_token_logprobs_bwd", dev, _lib.load().ada_token_logprobs_bwd, _lib.packed(logits),
+          _lib.packed(tokens), int(ignore_index), stats.data_ptr(), entropy.data_ptr(),
+          *(_lib.ptr(g) or None for g in ups), _lib.packed(grad))
     return grad
 
 
@@ -88,7 +92,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, ignore_index):
         z3 = _rows3(logits)
-        lp, ent, lse, top_lp, top_id, stats = _forward(z3, tokens, top_k, ignore_index)
+        lp, ent, lse, top_lp, top_id, stats = _forward(z3, tokens, top_k, ignore_index, views=False)
         ctx.save_for_backward(logits, tokens, stats, ent)
         ctx.ignore_index = ignore_index
         ctx.set_materialize_grads(False)

@@ -15,7 +15,7 @@ from serving_util import PoolModel, attend64, build_pool
 pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
 
 INVALID, SHAPE, DTYPE, LAYOUT, WORKSPACE, UNSUPPORTED = -1, -2, -3, -5, -8, -9
-T = _lib.tensor
+T = _lib.packed
 
 
 def _attn(q=None, k=None, v=None, table=None, lens=None, seqs=None, mask=None, ks=None, vs=None, out=None, ws=0):
