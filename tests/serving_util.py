@@ -32,7 +32,11 @@ def gather(pages, table_row, n, g):
     """The first n rows of head g of a sequence, 64-bit [n, D]."""
     page = pages.shape[2]
     ids = table_row[: (n + page - 1) // page].long()
-    return pages.float()[ids, g].double().reshape(-1, pages.shape[3])[:n]
+    if pages.element_size() == 1:  # 8-bit types are indexed as bytes
+        rows = pages.view(torch.uint8)[ids, g].view(pages.dtype)
+    else:
+        rows = pages[ids, g]
+    return rows.float().double().reshape(-1, pages.shape[3])[:n]
 
 
 def attend64(q, k, v, table, lens, scale, mask=None, ks=None, vs=None, seqs=None):

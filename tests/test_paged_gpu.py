@@ -126,6 +126,32 @@ def test_lowest_value_masks_leave_a_uniform_row(mdtype, cuda_device):
         assert (out.double() - want).abs().max().item() <= 2 * (math.exp(2.0 ** -8) - 1) * v.abs().max().item()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("mdtype", [torch.float32, torch.bfloat16])
+def test_lowest_value_masks_on_the_tensor_cores(mdtype, dtype, cuda_device):
+    """As above where the scores come from the tensor cores: -3.4e38 absorbs every score in fp32, all keys count alike."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(12)
+    k, v, table, ln = build_pool([50, 200], 16, 2, 64, dtype, g)
+    qd = torch.bfloat16 if dtype == torch.float8_e4m3fn else dtype
+    q = torch.randn(2, 4, 64, generator=g).to(qd)
+    m = torch.full((2, 200), torch.finfo(mdtype).min, dtype=mdtype)
+    out = ada.paged_attention(q.to(dev), k.to(dev), v.to(dev), table.to(dev), ln.to(dev), key_mask=m.to(dev)).cpu()
+    want, _ = attend64(torch.zeros_like(q), k, v, table, ln, 0.125)
+    err = (out.double() - want).abs()
+    assert (err <= _bar(torch.zeros_like(q), k, v, ln, 0.125, None, None, want)).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float8_e4m3fn, 128),
+                                     (torch.float8_e4m3fn, 64), (torch.float32, 64)])
+@pytest.mark.parametrize("b", [700, 4096])
+def test_large_batches(b, dtype, d, cuda_device):
+    """More sequences than a block has threads, and the most that a call takes (whose prefix leaves less shared memory)."""
+    g = torch.Generator().manual_seed(b)
+    lens = torch.randint(0, 41, (b,), generator=g).tolist()
+    _check(lens, 16, 2, 1, d, dtype, cuda_device, qdtype=None if dtype != torch.float8_e4m3fn else torch.bfloat16)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn])
 @pytest.mark.parametrize("shape", [(16, 4, 2, 128), (8, 2, 2, 64), (5, 4, 2, 96)])
