@@ -365,3 +365,35 @@ def test_refusals(cuda_device):
         ada.token_logprobs(z, t.cpu())
     with pytest.raises(Exception):
         ada.token_logprobs(z[:, :0], t)
+
+
+def _apart(z, t, dev, top):
+    """token_logprobs against 64 bits by a bar on z - max alone: the kernel's
+    sums hold exponents of x = z - max, and log p and H are differences of such.
+    log p adds the roundings of z_t - max and of the log, 2^-23 of their size;
+    only lse carries half a step of its own value."""
+    got = ada.token_logprobs(z.to(dev), t.to(dev), top_k=top)
+    lp, ent, lse, logp = _exact(z, t)
+    zf = z.double()
+    x = (zf.amax(-1) - zf.amin(-1)).max().item()
+    r = 2.0 ** -21 + min(x, 120.0) * 2.0 ** -23 + (z.shape[-1] / 256 + 40) * 2.0 ** -24
+    bar = 2 * r + 2.0 ** -22 * (min(x, 200.0) + math.log(z.shape[1]))
+    far = 2.0 ** -22 * lp.abs()  # a token far below the maximum
+    assert ((got.logprobs.cpu().double() - lp).abs() <= bar + far).all()
+    assert _off(got.entropy, ent) <= bar + 2 * r * (ent.max().item() + 1)
+    assert ((got.lse.cpu().double() - lse).abs() <= bar + 2.0 ** -23 * lse.abs()).all()
+    if top:
+        ids = _top(z, top)
+        assert torch.equal(got.top_tokens.cpu(), ids)
+        want = logp.gather(1, ids)
+        assert ((got.top_logprobs.cpu().double() - want).abs() <= bar + 2.0 ** -22 * want.abs()).all()
+    return got, bar, r
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset", [-3e4, -1e3, 1e3, 5e3, 3e4])
+@pytest.mark.parametrize("rows,vocab", [(3, 50257), (300, 5003)])
+def test_a_common_offset_costs_no_precision(rows, vocab, offset, dtype, cuda_device):
+    """Logits around +-10^3 to 3 10^4: their differences are as exact as without the offset."""
+    z, t = _make(rows, vocab, torch.float32)
+    _apart((z + offset).to(dtype), t, cuda_device, 5)
