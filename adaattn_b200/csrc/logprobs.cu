@@ -23,7 +23,7 @@
 // TB/s; fp32 473 us, 7.0 TB/s), 385 us with 5 and 437 us with 20 alternatives.
 // The gradient runs at 6.5 TB/s of reads and writes. Logits are clamped from below (-2^100;
 // fp16: its lowest value) so that -inf stays out of the weighted sum; a row
-// with nothing above the clamp is done again by the plain formulas.
+// whose maximum is beyond 2^15 in size is done again by the plain formulas.
 //
 // Top k (k <= 64): candidates are 64-bit keys, the value's order above the
 // inverted column, so all keys differ and equal values rank by lowest index.
@@ -166,11 +166,13 @@ template <int DT>
 __device__ __forceinline__ float lowest_kept() {
     return DT == ADA_F16 ? -65504.f : -1.2676506e30f;  // fp16's lowest value, -2^100
 }
-// A row maximum at which the clamp or m log2 e does not hold (NaN too).
-template <int DT>
-__device__ __forceinline__ bool ends_of_range(float m) {
-    return !(fabsf(m) <= -lowest_kept<DT>()) || m == lowest_kept<DT>();
-}
+// A row maximum far enough from 0 (NaN too) that the row takes the plain
+// formulas. The one-pass sums stand for exponents of x - M: M's rounding, up to
+// 2^-25 |M|, is in all of them until the end takes it out. Up to 2^15 that is at
+// most 2^-9 of an exponent; at 5e9 it passed 126 and the sums over- or
+// underflowed. It also keeps m so far above the clamp that what is clamped adds 0.
+constexpr float kFar = 32768.f;
+__device__ __forceinline__ bool ends_of_range(float m) { return !(fabsf(m) <= kFar); }
 template <int DT>
 __device__ __forceinline__ void unpack_pair(uint32_t w, float& lo, float& hi) {
     if constexpr (DT == ADA_BF16) {
@@ -277,7 +279,7 @@ __device__ __forceinline__ float add_round(PairSums& a, const uint32_t (&w)[Read
     return top;
 }
 
-// A row without a logit above the clamp, by the whole block: m, and s and t of x_i - m itself.
+// A row whose maximum is far from 0, by the whole block: m, and s and t of x_i - m itself.
 template <int DT>
 __device__ Sums plain_sums(const Reader<DT>& R, Sums* s_warp) {
     Sums a{-INFINITY, 0.f, 0.f};
@@ -617,10 +619,10 @@ __global__ void __launch_bounds__(kT, DT == ADA_F32 ? 0 : TOP ? 6 : 8) token_log
     }
     __syncthreads();
     a = s_part;
-    if (!ends_of_range<DT>(a.m) && threadIdx.x >= (TOP ? kMaxTop : 32)) return;
+    if (!ends_of_range(a.m) && threadIdx.x >= (TOP ? kMaxTop : 32)) return;
     // ls = log sum exp(z_i - m), mean = sum p_i (z_i - m), in base 2 first
     float ls, mean;
-    if (ends_of_range<DT>(a.m)) {
+    if (ends_of_range(a.m)) {
         a = plain_sums<DT>(R, s_warp);
         ls = logf(a.s);
         mean = a.t / a.s * kLn2;
@@ -671,7 +673,7 @@ __global__ void __launch_bounds__(kT) token_logprobs_bwd_kernel(const __grid_con
     const float c0 = g_lse - g_lp - g_h * L.entropy[row];
     const int rounds = R.rounds();
     // log2 p = (x - M) + shift with M as the forward's; rows near the ends of the range take the plain difference
-    const bool plain = ends_of_range<DT>(m);
+    const bool plain = ends_of_range(m);
     const float M = plain ? 0.f : m * kLog2e;
     const float shift = plain ? 0.f : -fmaf(ls, kLog2e, fmaf(m, kLog2e, -M));
     const uint64_t l2 = f2_splat(kLog2e), m2 = f2_splat(-M), sh2 = f2_splat(shift);

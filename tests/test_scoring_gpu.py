@@ -373,8 +373,10 @@ def _apart(z, t, dev, top):
     log p adds the roundings of z_t - max and of the log, 2^-23 of their size;
     only lse carries half a step of its own value."""
     got = ada.token_logprobs(z.to(dev), t.to(dev), top_k=top)
-    lp, ent, lse, logp = _exact(z, t)
     zf = z.double()
+    high = zf.amax(-1)
+    lp, ent, lse, logp = _exact(zf - high[:, None], t)  # (64 bits hold 10^15 to 0.125 only)
+    lse = lse + high
     x = (zf.amax(-1) - zf.amin(-1)).max().item()
     r = 2.0 ** -21 + min(x, 120.0) * 2.0 ** -23 + (z.shape[-1] / 256 + 40) * 2.0 ** -24
     bar = 2 * r + 2.0 ** -22 * (min(x, 200.0) + math.log(z.shape[1]))
@@ -397,3 +399,51 @@ def test_a_common_offset_costs_no_precision(rows, vocab, offset, dtype, cuda_dev
     """Logits around +-10^3 to 3 10^4: their differences are as exact as without the offset."""
     z, t = _make(rows, vocab, torch.float32)
     _apart((z + offset).to(dtype), t, cuda_device, 5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("level", [-1e4, 4e4, -1e6, -1e9, -1e10, 5e9, 1e15, -1e30, 1e38])
+def test_rows_far_from_zero(level, dtype, cuda_device):
+    """Constant rows, rows of two levels and rows that keep one large logit,
+    at sizes where max * log2(e) has no bits left for the exponents; with their gradient."""
+    dev = cuda_device
+    vocab = 9000
+    for rows in (4, 160):  # a cluster for each row, and a CTA
+        z = torch.full((rows, vocab), level, dtype=dtype)
+        z[1, 4000:] = level * (1 + 2.0 ** -7)  # another level, exactly held
+        z[2] = torch.randn(vocab, generator=torch.Generator().manual_seed(5)).to(dtype)
+        z[2, 77] = level
+        t = torch.arange(rows) * 7 % vocab
+        t[2] = 77
+        x = z.to(dev).requires_grad_()
+        got, bar, r = _apart(x.detach().cpu(), t, dev, 3)
+        out = ada.token_logprobs(x, t.to(dev))
+        for a, b in zip(out[:3], got[:3]):
+            assert (a - b).abs().max().item() <= 2 * bar + 2.0 ** -21 * b.abs().max().item()
+        g = torch.Generator().manual_seed(3)
+        ups = [torch.randn(rows, generator=g) for _ in range(3)]
+        grad, = torch.autograd.grad(out[:3], x, [u.to(dev) for u in ups])
+        zs = z.double() - z.double().amax(-1, keepdim=True)
+        want = _grad64(zs, t, *ups)
+        _, ent, _, logp = _exact(zs, t)
+        p = logp.exp()
+        size = p * (sum(u.abs().double() for u in ups)[:, None]
+                    * (1 + torch.where(p > 0, logp.abs(), torch.zeros_like(p)) + ent.abs()[:, None]))
+        hit = torch.zeros_like(want)
+        hit[torch.arange(rows), t] = ups[0].abs().double()
+        tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        slack = want.abs() * torch.finfo(dtype).eps / 2 + 4 * r * (size + hit) + tiny
+        assert ((grad.cpu().double() - want).abs() <= slack).all()
+
+
+def test_hidden_logits_beside_low_maxima(cuda_device):
+    """fp16 rows whose maximum is near the type's lowest value: what is -inf still has probability 0."""
+    dev = cuda_device
+    z = torch.full((2, 50000), -math.inf, dtype=torch.float16)
+    z[0, 9], z[1, 9], z[1, 12] = -65472.0, -65472.0, -65504.0
+    got = ada.token_logprobs(z.to(dev), torch.full((2,), 9, device=dev))
+    # one logit: exactly 0; two, 32 apart: p = e^-32, H = log s + 32 p with s = 1 + e^-32, which fp32
+    # rounds to 1: log s is 0 in place of e^-32, and the rest is off by fp32 roundings
+    assert got.logprobs.tolist()[0] == 0 and got.entropy.tolist()[0] == 0
+    p = math.exp(-32)
+    assert abs(got.logprobs[1].item()) <= 1e-13 and abs(got.entropy[1].item() - 33 * p) <= p + 33 * p * 1e-5
