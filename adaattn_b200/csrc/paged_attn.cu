@@ -538,9 +538,13 @@ int launch_simt_gb(const PagedAttnLaunch& L, cudaStream_t stream) {
 // padding the heads to a 128-row tile would leave most of it empty. Scores
 // come out with a key per row; an 8 x 8 transpose in registers (movmatrix)
 // turns P into the next product's operand. P enters as two 16-bit parts
-// (hi + lo, 16 bits for bf16 and 22 for fp16), so that only the output is
-// rounded. 8-bit pages become fp16 operands in registers: E4M3 values are fp16
-// values, q is scaled into fp16's range by a power of two per head. The order
+// hi + lo: 16 bits of it for bf16, 22 for fp16. fp16 ends at 2^-24, so there p
+// carries a factor 2^15 (p <= 2^15 fits) until the sums leave the warp, and what
+// is lost of a p is at most 2^-40 of the largest: without it a tail 17 below an
+// attention sink's score, whose own value is near 0, came out as nothing.
+// 8-bit pages become fp16 operands in registers: E4M3 values are fp16
+// values, q is scaled into fp16's range by a power of two per head (elements
+// below 2^-14 of the head's largest lose bits to fp16's end). The order
 // of elements within a head is free as long as K and q agree on it, and V's
 // with the output, so 4 consecutive bytes of a row serve two k positions.
 //
@@ -561,6 +565,9 @@ struct TcCfg {
     static constexpr int STAGES = TILE >= 8192 ? 3 : 6;      // at most; fewer when the rest needs the space
     static constexpr int GB = 8 * NT;
     static constexpr int PART = GB * D;                      // floats a warp leaves per slot
+    // the exponent that p carries on its way through fp16 operands
+    static constexpr float LIFT = KIND == 0 ? 0.f : 15.f;
+    static constexpr float DROP = KIND == 0 ? 1.f : 1.f / 32768.f;
     // beside the ring: slot 0 of the join (slot 1 lies in the drained ring) and (m, l)
     static constexpr int BESIDE = WARPS * (PART * 4 + 2 * GB * 2 * 4);
 };
@@ -945,8 +952,8 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                 for (int r = 0; r < 2; ++r)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float p0 = fast_exp2((c[r][n][2 * j] - ref[0]) * unit);
-                        const float p1 = fast_exp2((c[r][n][2 * j + 1] - ref[1]) * unit);
+                        const float p0 = fast_exp2(fmaf(c[r][n][2 * j] - ref[0], unit, C::LIFT));
+                        const float p1 = fast_exp2(fmaf(c[r][n][2 * j + 1] - ref[1], unit, C::LIFT));
                         l[n][0] += p0;
                         l[n][1] += p1;
                         uint32_t hi, lo;
@@ -1013,6 +1020,7 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                 sum += __shfl_xor_sync(0xffffffffu, sum, 4);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                sum *= C::DROP;
                 const int h = n * 8 + 2 * ft + e;
                 if (h >= heads) continue;
                 const float inv = whole ? (sum == 0.f ? 0.f : vs / sum) : 1.f;
@@ -1022,7 +1030,7 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const int d = KIND == 2 ? i * 16 + 2 * fg + j : i * 16 + fg + 8 * j;
-                        const float v = sum == 0.f ? 0.f : o[i][n][2 * j + e] * inv;
+                        const float v = sum == 0.f ? 0.f : o[i][n][2 * j + e] * C::DROP * inv;
                         if (whole) store_out(L, x.b, h0 + h, d, v);
                         else part[h * D + d] = v;
                     }

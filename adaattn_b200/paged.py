@@ -98,7 +98,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (True keeps) or floating point (added; -inf hides); later keys are open
     and hidden keys are not read. ``scale`` defaults to D ** -0.5.
 
-    Scores, softmax and sums are fp32, the result is rounded once. A sequence
+    Scores, softmax and sums are fp32, the result is rounded once. On the
+    tensor cores (16- and 8-bit pages, heads of 64 or 128) a probability is
+    held to 16 bits over bf16 pages, to 22 bits and 2^-40 of the largest one
+    over the others, and q over 8-bit pages to fp16's bits after a power of two
+    per head; a visible infinite value may come out as NaN there. A sequence
     without a visible key gives zeros. With ``return_lse`` also the fp32
     [B, H] log-sum-exp of the scores (-inf there). No autograd. Up to 4096
     sequences per call, head dims up to 128.

@@ -434,3 +434,37 @@ def test_append_picks_refuses_and_bounds(cuda_device):
         ada.paged_append(k.to(dev).half(), k.to(dev).half(), kp.to(dev), vp.to(dev), table.to(dev), ln.to(dev))
     with pytest.raises(ada.ShapeError):
         ada.paged_append(k.to(dev)[:, :1], k.to(dev)[:, :1], kp.to(dev), vp.to(dev), table.to(dev), ln.to(dev))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float8_e4m3fn, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("group", [1, 16])
+@pytest.mark.parametrize("above", [14.0, 18.0, 20.0])
+def test_what_stands_behind_an_attention_sink_is_kept(above, group, d, dtype, cuda_device):
+    """One key with a score far above all others and a value of 0 (a sink): the
+    output is the others' sum alone, (n - 1) e^-a / (1 + (n - 1) e^-a). A
+    probability enters a 16-bit product with 2^-16 of itself (bf16) or with
+    2^-22 of itself and 2^-40 of the largest one (fp16), the fp32 exponent and
+    exponential add 2^-19, the output half a step (below the type's normal
+    values, as fp16's output at 20 is, half of its smallest). 300 sequences of 4096 keys
+    (over the same pages) make units that one warp takes whole: its sums of n
+    equal terms take up to n dependent fp32 additions, each off by at most 2^-24
+    of a running sum that is no larger than the final one, n 2^-24 in all. The
+    sum of p has the same error, lse that much absolutely beside its own 2^-23."""
+    dev = cuda_device
+    n, page, hkv, b = 4096, 64, 4, 300
+    k, v = torch.zeros(n // page, hkv, page, d), torch.ones(n // page, hkv, page, d)
+    k[0, :, 0, 0], v[0, :, 0] = above, 0.0
+    qd = torch.bfloat16 if dtype == torch.float8_e4m3fn else dtype
+    q = torch.zeros(b, hkv * group, d, dtype=qd)
+    q[:, :, 0] = 1.0
+    table = torch.arange(n // page, dtype=torch.int32).expand(b, -1).contiguous()
+    ln = torch.full((b,), n, dtype=torch.int32)
+    out, lse = ada.paged_attention(q.to(dev), k.to(dtype).to(dev), v.to(dtype).to(dev), table.to(dev), ln.to(dev),
+                                   scale=1.0, return_lse=True)
+    rest = (n - 1) * math.exp(-above)
+    want = rest / (1 + rest)
+    lost = {torch.bfloat16: 2.0 ** -16, torch.float32: 0.0}.get(dtype, 2.0 ** -22 + 2.0 ** -40 * math.exp(above))
+    step = torch.finfo(qd).smallest_normal * HALF[qd]
+    assert (out.double() - want).abs().max().item() <= step + want * (HALF[qd] + lost + 2.0 ** -19 + n * 2.0 ** -24)
+    assert (lse.double() - above - math.log1p(rest)).abs().max().item() <= 2.0 ** -19 + n * 2.0 ** -24 + 2.0 ** -23 * above
