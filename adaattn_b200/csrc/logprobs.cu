@@ -333,7 +333,9 @@ struct TopState {
     uint32_t digit, below;
 };
 
-// Of a thread's rounds: the three largest maxima and the rounds of the first two.
+// Of a thread's rounds: the three largest maxima and the rounds of the first
+// two. A NaN gives way to the next round's maximum and steps down a place; it
+// stays among the three, as `third` keeps NaN, so top and second together show it.
 struct Seen {
     float top, second, third;
     int round, round2;
@@ -459,7 +461,7 @@ __device__ void best_keys(TopState& S, int k, const Seen& mine, const Reader<DT>
         // read the elements of the best round, the others those of the second.
         const int half = lane >> 4, e = lane & 15;
         const int at = (e / EPV) * kT * EPV + e % EPV - lane * EPV + R.c0;
-        uint32_t todo = __ballot_sync(0xffffffffu, order_of(mine.top) >= bound);
+        uint32_t todo = __ballot_sync(0xffffffffu, order_of(max_nan(mine.top, mine.second)) >= bound);
         const uint32_t more = __ballot_sync(0xffffffffu, order_of(mine.second) >= bound);
         while (todo != 0) {
             float x[4];

@@ -447,3 +447,18 @@ def test_hidden_logits_beside_low_maxima(cuda_device):
     assert got.logprobs.tolist()[0] == 0 and got.entropy.tolist()[0] == 0
     p = math.exp(-32)
     assert abs(got.logprobs[1].item()) <= 1e-13 and abs(got.entropy[1].item() - 33 * p) <= p + 33 * p * 1e-5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,top", [(200, 6000, 3), (200, 6000, 40), (16, 50257, 3), (2, 131072, 20)])
+def test_nan_comes_first_wherever_it_stands(rows, vocab, top, dtype, cuda_device):
+    """One NaN a row, in a thread's first, middle or last round: it is the first alternative, the others follow in order."""
+    z, _ = _make(rows, vocab, dtype, spread=1.0)
+    at = torch.arange(rows) * 997 % vocab
+    at[::3] = torch.arange(rows)[::3] % 64  # first rounds
+    at[1::3] = vocab - 1 - torch.arange(rows)[1::3] % 64
+    z[torch.arange(rows), at] = math.nan
+    got = ada.token_logprobs(z.to(cuda_device), torch.zeros(rows, dtype=torch.int64, device=cuda_device), top_k=top)
+    assert torch.equal(got.top_tokens[:, 0].cpu(), at)
+    assert torch.equal(got.top_tokens[:, 1:].cpu(), _top(z.nan_to_num(nan=-math.inf), top - 1))
+    assert torch.isnan(got.logprobs).all() and torch.isnan(got.top_logprobs).all()
