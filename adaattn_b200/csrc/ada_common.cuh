@@ -131,6 +131,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         }
     }
 }
+// The same for a whole warp, with one answer: its lanes look at the barrier, the
+// clock and the abort flag each for itself, and where one gave up while another
+// saw the phase complete, the two would meet different warp-wide exchanges.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                               uint64_t timeout_ns, unsigned int* status) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, timeout_ns, status));
+}
 
 // ---------------------------------------------------------------------------
 // TMA (no cluster multicast anywhere in this library).

@@ -541,19 +541,25 @@ __global__ void target_ranks_kernel(const float* eff, int64_t n, int64_t min_ran
     }
 }
 
-// Waits on a barrier nothing signals; the bounded wait gives up and records
-// ADA_ERR_TIMEOUT, after which the kernel returns normally.
+// One warp waits on a barrier nothing signals; the bounded wait gives up and
+// records ADA_ERR_TIMEOUT, after which the kernel returns normally. Half of its
+// lanes wait for a phase that is complete: the warp's wait gives all lanes one
+// answer all the same (ADA_ERR_INVALID is recorded if it does not).
 __global__ void bounded_wait_kernel(uint64_t timeout_ns, unsigned int* status) {
-    __shared__ __align__(8) uint64_t bar;
+    __shared__ __align__(8) uint64_t bar[2];
     __shared__ int abort_flag;
     if (threadIdx.x == 0) {
-        mbar_init(smem_u32(&bar), 1);
+        mbar_init(smem_u32(&bar[0]), 1);
+        mbar_init(smem_u32(&bar[1]), 1);
         abort_flag = 0;
         fence_mbar_init();
+        mbar_arrive(smem_u32(&bar[1]));
     }
     __syncthreads();
-    if (threadIdx.x == 0) mbar_wait(smem_u32(&bar), 0, &abort_flag, timeout_ns, status);
-    __syncthreads();
+    const bool ok = mbar_wait_warp(smem_u32(&bar[threadIdx.x & 1]), 0, &abort_flag, timeout_ns, status);
+    __syncwarp();
+    const uint32_t saw = __ballot_sync(0xffffffffu, ok);
+    if (threadIdx.x == 0 && saw != 0u) record_error(status, ADA_ERR_INVALID);
 }
 
 }  // namespace

@@ -848,7 +848,7 @@ __global__ void __launch_bounds__(TcCfg<KIND, D, NT>::WARPS * 32, 1)
                     add = open ? mv : 0.f;
                 }
             }
-            if (!mbar_wait(bar0 + slot * 8, parity, abort_flag, limit, status)) {
+            if (!mbar_wait_warp(bar0 + slot * 8, parity, abort_flag, limit, status)) {
                 alive = false;
                 break;
             }

@@ -43,3 +43,17 @@ def test_host_side_argument_errors(cuda_device):
     big = torch.randn(1, 1, 16, 160, device=cuda_device)
     with pytest.raises(KernelError):
         attention_forward(big, big, big, scale=0.1, static_precision=PrecisionMode.FP32)
+
+
+def test_a_warps_wait_has_one_answer(cuda_device):
+    """Lanes of one warp that see a phase complete give up with those that time
+    out (the test kernel records code -1 where they do not), from the shortest limits on."""
+    lib = _lib.load()
+    _lib.poll_device_status(cuda_device)
+    with torch.cuda.device(cuda_device):
+        for limit_ns in (1, 1000, 50_000, 1_000_000):
+            for _ in range(5):
+                assert lib.ada_debug_bounded_wait(limit_ns, _lib.stream_ptr(cuda_device)) == 0
+                with pytest.raises(KernelError) as e:
+                    _lib.poll_device_status(cuda_device)
+                assert e.value.code == -7
