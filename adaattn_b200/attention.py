@@ -29,6 +29,7 @@ from torch import Tensor
 from . import core
 from .config import (AttentionConfig, MemoryError, NumericalError, PrecisionMode,
                      ShapeError)
+from .paged import _no_tangent
 
 logger = logging.getLogger(__name__)
 
@@ -283,6 +284,7 @@ class AdaAttention(nn.Module):
         if x.ndim != 3 or x.shape[-1] != self.embed_dim:
             raise ShapeError("x must be [B, N, E]", expected_shape=(None, None, self.embed_dim),
                              actual_shape=tuple(x.shape))
+        _no_tangent("cached decoding", x, residual)
         b, n, e = x.shape
         h, d = self.num_heads, self.head_dim
         with torch.no_grad():

@@ -20,6 +20,7 @@ import functools
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from . import _lib
 from .config import ShapeError
@@ -49,7 +50,15 @@ def _device_of(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> torch.devi
     return first.device
 
 
+def _no_tangent(what: str, *ts: Optional[torch.Tensor]) -> None:
+    """Refuses dual tensors, whose tangents the kernels would drop (they need no requires_grad)."""
+    if _fwd._current_level >= 0 and any(
+            t is not None and t.is_floating_point() and _fwd.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{what} has no forward-mode derivative: call it outside dual levels or on the primals")
+
+
 def _no_grad(what: str, *ts: Optional[torch.Tensor]) -> None:
+    _no_tangent(what, *ts)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
@@ -109,6 +118,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """
     dev = _device_of(q, k_pages, v_pages, page_table, seq_lens, seqs, key_mask, k_scale, v_scale, out)
     _no_grad("paged_attention", q, k_pages, v_pages, key_mask)
+    _no_tangent("paged_attention", k_scale, v_scale)
     if q.dim() != 3:
         raise ShapeError(f"q must be 3-D [B, H, D], got {q.dim()}-D")
     if k_pages.dim() != 4:
@@ -145,6 +155,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     """
     dev = _device_of(k, v, k_pages, v_pages, page_table, seq_lens, new_tokens, seqs, k_scale, v_scale)
     _no_grad("paged_append", k, v, k_pages, v_pages)
+    _no_tangent("paged_append", k_scale, v_scale)
     _call("ada_paged_append", dev, _lib.load().ada_paged_append, _lib.packed(_unit_last(k)),
           _lib.packed(_unit_last(v)), _lib.packed(k_pages), _lib.packed(v_pages), _lib.packed(page_table),
           _lib.packed(seq_lens), _opt(new_tokens), _opt(seqs), _opt(k_scale), _opt(v_scale))

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from .config import ShapeError
-from .paged import _call, _device_of
+from .paged import _call, _device_of, _no_tangent
 
 
 class TokenLogprobs(NamedTuple):
@@ -81,6 +81,7 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, stats: t
     logits' padding in memory."""
     ups = [None if g is None else g.float().contiguous() for g in (grad_logprobs, grad_entropy, grad_lse)]
     dev = _device_of(logits, tokens, stats, entropy, *ups)
+    _no_tangent("token_logprobs_backward", logits, stats, entropy, *ups)
     grad = _grad_like(logits)
     _call("ada_token_logprobs_bwd", dev, _lib.load().ada_token_logprobs_bwd, _lib.packed(logits),
           _lib.packed(tokens), int(ignore_index), stats.data_ptr(), entropy.data_ptr(),
@@ -125,10 +126,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top_k: int = 0
     nothing else, or one with +inf or NaN, gives NaN.
 
     logprobs, entropy and lse are differentiable with respect to the logits
-    (once); the gradient has their dtype. An entropy gradient reaches ignored
+    (once, in reverse mode; dual tensors are refused); the gradient has their dtype. An entropy gradient reaches ignored
     rows too.
     """
     dev = _device_of(logits, tokens)
+    _no_tangent("token_logprobs", logits)
     if logits.dim() < 1:
         raise ShapeError("logits must be [..., V]")
     if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):

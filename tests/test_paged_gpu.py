@@ -468,3 +468,29 @@ def test_what_stands_behind_an_attention_sink_is_kept(above, group, d, dtype, cu
     step = torch.finfo(qd).smallest_normal * HALF[qd]
     assert (out.double() - want).abs().max().item() <= step + want * (HALF[qd] + lost + 2.0 ** -19 + n * 2.0 ** -24)
     assert (lse.double() - above - math.log1p(rest)).abs().max().item() <= 2.0 ** -19 + n * 2.0 ** -24 + 2.0 ** -23 * above
+
+
+def test_forward_mode_is_refused(cuda_device):
+    fwd = torch.autograd.forward_ad
+    dev = cuda_device
+    g = torch.Generator().manual_seed(13)
+    k, v, table, ln = (t.to(dev) for t in build_pool([20], 16, 2, 64, torch.float32, g))
+    q = torch.randn(1, 4, 64, generator=g).to(dev)
+    m = torch.zeros(1, 20, device=dev)
+    new = torch.randn(1, 2, 1, 64, generator=g).to(dev)
+    want = ada.paged_attention(q, k, v, table, ln, key_mask=m)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for args, kw in (((dual(q), k, v), {}), ((q, dual(k), v), {}), ((q, k, dual(v)), {}),
+                         ((q, k, v), dict(key_mask=dual(m)))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ada.paged_attention(*args, table, ln, **kw)
+        before = k.clone()
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ada.paged_append(dual(new), new, k, v, table, ln)
+        assert torch.equal(k, before)
+        assert torch.equal(ada.paged_attention(q, k, v, table, ln, key_mask=m), want)
+        c = ada.PagedKVCache(1, 4, 8, 2, 32, max_sequences=1, max_pages_per_sequence=4)
+        att = ada.AdaAttention(embed_dim=64, num_heads=2, causal=True, enable_adaptive_rank=False).to(dev).eval()
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            att.forward_cached(dual(torch.randn(1, 1, 64, device=dev)), c, 0)

@@ -462,3 +462,25 @@ def test_nan_comes_first_wherever_it_stands(rows, vocab, top, dtype, cuda_device
     assert torch.equal(got.top_tokens[:, 0].cpu(), at)
     assert torch.equal(got.top_tokens[:, 1:].cpu(), _top(z.nan_to_num(nan=-math.inf), top - 1))
     assert torch.isnan(got.logprobs).all() and torch.isnan(got.top_logprobs).all()
+
+
+def test_forward_mode_is_refused(cuda_device):
+    """A dual tensor does not require grad; its tangent is not dropped without a word."""
+    fwd = torch.autograd.forward_ad
+    dev = cuda_device
+    z, t = _make(4, 50, torch.float32)
+    z, t = z.to(dev), t.to(dev)
+    want = ada.token_logprobs(z, t)
+    ones = torch.ones(4, device=dev)
+    stats = torch.stack([z.amax(-1), want.lse - z.amax(-1)], 1)
+    with fwd.dual_level():
+        dual = fwd.make_dual(z, torch.ones_like(z))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ada.token_logprobs(dual, t)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            token_logprobs_backward(z[None], t, stats, want.entropy, fwd.make_dual(ones, ones))
+        with pytest.raises(RuntimeError):
+            ada.token_logprobs(fwd.make_dual(z.clone().requires_grad_(), torch.ones_like(z)), t)
+        assert torch.equal(ada.token_logprobs(z, t).logprobs, want.logprobs)  # no tangent here
+    with pytest.raises(Exception):
+        torch.func.jvp(lambda x: ada.token_logprobs(x, t).lse, (z,), (z,))
