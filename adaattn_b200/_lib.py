@@ -92,6 +92,7 @@ _SIGNATURES = {
     "ada_paged_attn": (c_int32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_float, _P, c_void_p, c_void_p,
                                  c_size_t, c_void_p]),
     "ada_paged_append": (c_int32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_void_p]),
+    "ada_paged_append_prompts": (c_int32, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_void_p]),
     "ada_pages_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "ada_pages_free": (c_int32, [_P, _P, _P, c_int64, _P, c_void_p]),
     "ada_pages_fork": (c_int32, [_P, _P, _P, c_int64, _P, _P, c_void_p]),

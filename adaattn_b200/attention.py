@@ -268,7 +268,10 @@ class AdaAttention(nn.Module):
         N = 1: each token attends to its sequence's whole cache
         (``paged_attention``). N > 1: the prompts of sequences that hold
         nothing else, right-padded to N with new_tokens[b] real tokens each
-        (N when omitted), run through the causal attention of ``forward``.
+        (N when omitted), run through the causal attention of ``forward``. A
+        sequence that holds tokens already is recorded in the library's status
+        word (``_lib.poll_device_status`` raises), nothing is appended to it and
+        its rows mean nothing: its tokens go one by one.
         Heads are dense: the module must be causal and built with
         ``enable_adaptive_rank=False``, since a low-rank decision taken for a
         prompt has no counterpart over the cache. Inference only (eval mode,
@@ -292,7 +295,7 @@ class AdaAttention(nn.Module):
             qkv = (core.linear(x, w, bias) if self._dense_on_tensor_cores(x)
                    else torch.nn.functional.linear(x, w, bias))
             q, k, v = (qkv[..., i * e:(i + 1) * e].view(b, n, h, d).transpose(1, 2) for i in range(3))
-            cache.append(layer, k, v, new_tokens, seqs=seqs)
+            cache.append(layer, k, v, new_tokens, seqs=seqs, prompts=n > 1)
             if n == 1:
                 merged = cache.attend(layer, q[:, :, 0], seqs=seqs, scale=self.scale).view(b, 1, e)
             else:

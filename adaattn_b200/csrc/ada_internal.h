@@ -358,6 +358,7 @@ struct AppendLaunch {
     int page, D;
     int vec;             // rows of both sides aligned for eight elements, D a multiple of 8
     int chunks;          // blocks per sequence
+    int prompts;         // 1: a sequence must hold its new tokens only
     const float* k_scale;
     const float* v_scale;
     unsigned int* status;

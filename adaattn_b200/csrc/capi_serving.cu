@@ -403,9 +403,10 @@ int ada_paged_attn(const AdaTensor* q, const AdaTensor* k_pages, const AdaTensor
     return rc ? fail(rc, "paged attention launch failed: %s", cudaGetErrorString(cudaGetLastError())) : ADA_OK;
 }
 
-int ada_paged_append(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages, AdaTensor* v_pages,
-                     const AdaTensor* page_table, const AdaTensor* seq_lens, const AdaTensor* new_tokens,
-                     const AdaTensor* seqs, const AdaTensor* k_scale, const AdaTensor* v_scale, void* stream) {
+namespace {
+int append(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages, AdaTensor* v_pages, const AdaTensor* page_table,
+           const AdaTensor* seq_lens, const AdaTensor* new_tokens, const AdaTensor* seqs, const AdaTensor* k_scale,
+           const AdaTensor* v_scale, bool prompts, void* stream) {
     int rc;
     if ((rc = check_view(k, "k", 4)) || (rc = check_view(v, "v", 4))) return rc;
     if (!is_float(k->dtype)) return fail(ADA_ERR_DTYPE, "k must be fp32, fp16 or bf16");
@@ -470,8 +471,22 @@ int ada_paged_append(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages,
     const int64_t most = std::max<int64_t>(1, int64_t(sms) * 16 / B);
     L.chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((N + at_once - 1) / at_once, most)));
     if (B * L.chunks > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "too many sequences");
+    L.prompts = prompts;
     rc = launch_paged_append(L, static_cast<cudaStream_t>(stream));
     return rc ? fail(rc, "append launch failed: %s", cudaGetErrorString(cudaGetLastError())) : ADA_OK;
+}
+}  // namespace
+
+int ada_paged_append(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages, AdaTensor* v_pages,
+                     const AdaTensor* page_table, const AdaTensor* seq_lens, const AdaTensor* new_tokens,
+                     const AdaTensor* seqs, const AdaTensor* k_scale, const AdaTensor* v_scale, void* stream) {
+    return append(k, v, k_pages, v_pages, page_table, seq_lens, new_tokens, seqs, k_scale, v_scale, false, stream);
+}
+
+int ada_paged_append_prompts(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages, AdaTensor* v_pages,
+                             const AdaTensor* page_table, const AdaTensor* seq_lens, const AdaTensor* new_tokens,
+                             const AdaTensor* seqs, const AdaTensor* k_scale, const AdaTensor* v_scale, void* stream) {
+    return append(k, v, k_pages, v_pages, page_table, seq_lens, new_tokens, seqs, k_scale, v_scale, true, stream);
 }
 
 size_t ada_pages_workspace_bytes(int64_t num_pages, int64_t num_sequences, int64_t n) {

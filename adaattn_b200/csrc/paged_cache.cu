@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged_append_kernel(const _
     if (!bad) {
         len = L.lens[r];
         n = L.new_tokens != nullptr ? L.new_tokens[b] : L.N;
-        bad = n < 0 || n > L.N || len < n || len > L.W * L.page;
+        bad = n < 0 || n > L.N || len < n || len > L.W * L.page || (L.prompts != 0 && n > 0 && len != n);
     }
     if (bad) {
         if (threadIdx.x == 0) record_error(L.status, ADA_ERR_INVALID);

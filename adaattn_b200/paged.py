@@ -142,7 +142,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                  page_table: torch.Tensor, seq_lens: torch.Tensor,
                  new_tokens: Optional[torch.Tensor] = None, *, seqs: Optional[torch.Tensor] = None,
-                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
+                 k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                 prompts: bool = False) -> None:
     """Write new keys and values into their pages in place (``ada_paged_append``).
 
     k, v [B, Hkv, N, D] views (unit innermost stride): token t <
@@ -152,11 +153,15 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     them. The pages written must be held by their sequence alone (which
     ``reserve_pages`` sees to). k and v have the pages' dtype, or the pages are
     float8_e4m3fn and receive value / scale, rounded once and saturated at 448.
+    With ``prompts`` the new tokens must be all that their sequence holds; one
+    that holds others too is left out and recorded in the status word.
     """
     dev = _device_of(k, v, k_pages, v_pages, page_table, seq_lens, new_tokens, seqs, k_scale, v_scale)
     _no_grad("paged_append", k, v, k_pages, v_pages)
     _no_tangent("paged_append", k_scale, v_scale)
-    _call("ada_paged_append", dev, _lib.load().ada_paged_append, _lib.packed(_unit_last(k)),
+    lib = _lib.load()
+    _call("ada_paged_append", dev, lib.ada_paged_append_prompts if prompts else lib.ada_paged_append,
+          _lib.packed(_unit_last(k)),
           _lib.packed(_unit_last(v)), _lib.packed(k_pages), _lib.packed(v_pages), _lib.packed(page_table),
           _lib.packed(seq_lens), _opt(new_tokens), _opt(seqs), _opt(k_scale), _opt(v_scale))
 
@@ -330,11 +335,11 @@ class PagedKVCache:
         return reserve_pages(self.data, *self._pool(), _ids(seqs, self.device), _ids(new_tokens, self.device))
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, new_tokens: Optional[Ids] = None, *,
-               seqs: Optional[Ids] = None) -> None:
+               seqs: Optional[Ids] = None, prompts: bool = False) -> None:
         """Write k, v [B, Hkv, N, D] of the newest tokens of seqs (``paged_append``)."""
         paged_append(k, v, self.keys(layer), self.values(layer), self.page_table, self.seq_lens,
                      None if new_tokens is None else _ids(new_tokens, self.device),
-                     seqs=None if seqs is None else _ids(seqs, self.device), **self._scales(layer))
+                     seqs=None if seqs is None else _ids(seqs, self.device), prompts=prompts, **self._scales(layer))
 
     def attend(self, layer: int, q: torch.Tensor, *, seqs: Optional[Ids] = None, **kwargs):
         """Attention of q [B, H, D], the newest tokens of seqs, over the layer's cache (``paged_attention``)."""

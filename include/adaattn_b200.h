@@ -321,6 +321,13 @@ int         ada_paged_append(const AdaTensor* k, const AdaTensor* v, AdaTensor* 
                              const AdaTensor* page_table, const AdaTensor* seq_lens,
                              const AdaTensor* new_tokens, const AdaTensor* seqs,
                              const AdaTensor* k_scale, const AdaTensor* v_scale, void* stream);
+/* The same for the tokens of prompts, whose attention runs over them alone: a
+ * sequence that holds anything else (seq_lens other than new_tokens, unless
+ * that is 0) is left out and recorded. */
+int         ada_paged_append_prompts(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages, AdaTensor* v_pages,
+                                     const AdaTensor* page_table, const AdaTensor* seq_lens,
+                                     const AdaTensor* new_tokens, const AdaTensor* seqs,
+                                     const AdaTensor* k_scale, const AdaTensor* v_scale, void* stream);
 
 /* Page operations. `pages` is the page data [planes, P, elements of a page]
  * (a plane per layer and tensor). Free pages are handed out lowest id first.

@@ -221,3 +221,45 @@ def test_refusals(cuda_device):
         m.eval().forward_cached(x[..., :32], c, 0)
     with pytest.raises(IndexError):
         m.forward_cached(x, c, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_several_tokens_after_cached_ones_are_recorded(dtype, cuda_device):
+    """N > 1 attends within its own tokens: a sequence that holds others is left
+    out and recorded, its neighbours in the batch and empty rows are not; token by token it goes on."""
+    dev = cuda_device
+    prec = {torch.float32: PrecisionMode.FP32, torch.bfloat16: PrecisionMode.BF16}[dtype]
+    att = ada.AdaAttention(embed_dim=E, num_heads=H, causal=True, enable_adaptive_rank=False, dropout=0.0,
+                           enable_adaptive_precision=False, default_precision=prec).to(dev).to(dtype).eval()
+    x = torch.randn(3, 12, E, generator=torch.Generator().manual_seed(8)).to(dev).to(dtype)
+    cache = ada.PagedKVCache(1, 16, 8, H, E // H, max_sequences=4, max_pages_per_sequence=4, dtype=dtype)
+    cache.reserve([0], [5])
+    att.forward_cached(x[:1, :5], cache, 0, seqs=_ids([0], dev))
+    _lib.poll_device_status(dev)
+    # row 0 holds five tokens; row 2 is new; row 3 takes part with no token at all
+    cache.reserve([0, 2], [7, 12])
+    before, full = cache.data.clone(), att.forward_cached(x[1:2], _fresh(cache), 0, seqs=_ids([1], dev))
+    got = att.forward_cached(x, cache, 0, seqs=_ids([0, 2, 3], dev), new_tokens=_ids([7, 12, 0], dev))
+    with pytest.raises(ada.KernelError):
+        _lib.poll_device_status(dev)
+    # (the library's fp32 products add 256 terms in another order for another batch)
+    tol = {torch.bfloat16: 2.0 ** -7, torch.float32: 1e-5}[dtype]
+    assert (got[1].float() - full[0].float()).abs().max().item() <= tol * full.float().abs().max().item()
+    pages = cache.page_table[0, :2].long()
+    assert torch.equal(cache.data[:, pages], before[:, pages])
+    # the refused tokens one by one, as the documentation puts it
+    cache.free([0])
+    whole = att(x[:1], x[:1], x[:1])[0]
+    for t in range(12):
+        cache.reserve([0], [1])
+        y = att.forward_cached(x[:1, t:t + 1], cache, 0, seqs=_ids([0], dev))
+        assert (y[0, 0].float() - whole[0, t].float()).abs().max().item() <= tol * whole.float().abs().max().item()
+    _lib.poll_device_status(dev)
+
+
+def _fresh(cache):
+    """A cache of the same shape with room for 12 tokens in row 1."""
+    p, hkv, page, d = cache.data.shape[1:]
+    c = ada.PagedKVCache(1, p, page, hkv, d, max_sequences=4, max_pages_per_sequence=4, dtype=cache.dtype)
+    c.reserve([1], [12])
+    return c
