@@ -365,6 +365,7 @@ struct AppendLaunch {
 };
 int launch_paged_append(const AppendLaunch& L, cudaStream_t stream);
 
+constexpr int kMaxNeed = (1 << 29) - 1;  // pages that a sequence may need, a copy of its last one among them
 struct PagesLaunch {
     int32_t* table;      // [S, W] rows at table_ld
     int32_t* lens;       // [S]

@@ -199,6 +199,9 @@ int pages_table(const AdaTensor* table, const AdaTensor* lens, const AdaTensor* 
     // the pages that a call can need are counted in 32 bits
     if (table->shape[0] * (table->shape[1] + 1) > kMaxInt)
         return fail(ADA_ERR_UNSUPPORTED, "page_table has 2^31 or more entries");
+    // and a sequence's share the word with two flags (kNeed)
+    if (table->shape[1] >= kMaxNeed)
+        return fail(ADA_ERR_UNSUPPORTED, "at most 2^29 - 2 page_table entries per sequence");
     if (table->shape[0] > 1 && table->stride[0] < table->shape[1])
         return fail(ADA_ERR_LAYOUT, "the rows of page_table overlap");
     *L = PagesLaunch{};

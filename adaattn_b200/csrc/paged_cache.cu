@@ -277,6 +277,7 @@ __device__ int block_scan(int x, int* total, int* sums) {
 // or when the needs up to and including its own fit the free pages; another is
 // left as it was (reserve) or empty (copy). The pages to copy go to L.pairs.
 constexpr int kCopies = 1 << 30, kKeeps = 1 << 29, kNeed = kKeeps - 1;  // flags beside a need
+static_assert(kNeed == kMaxNeed, "a need with its flags");
 
 template <bool COPY>
 __global__ void __launch_bounds__(kAllocThreads) pages_alloc_kernel(const __grid_constant__ PagesLaunch L) {

@@ -292,7 +292,8 @@ int         ada_record_statistics(const float* summary, AdaTensor* call_count,
  * wrong in device data (a page id, a length, a sequence or a token out of
  * range) it leaves out, and records ADA_ERR_INVALID in the status word that
  * ada_poll_device_status reads. Views with at most 2^30 pages and 2^31 - 1
- * tokens per sequence, table entries and rows; head dims 1..128; pages of
+ * tokens per sequence, table entries and rows (the page operations: 2^29 - 2
+ * table entries per sequence); head dims 1..128; pages of
  * 1..65536 tokens. */
 
 /* out[b, h] = softmax(scale * q[b, h] . K) V over the seq_lens keys of table

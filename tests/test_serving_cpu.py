@@ -130,6 +130,28 @@ def test_page_operations_refuse_before_any_device_work():
         _planes(data.transpose(3, 4))
 
 
+def test_needs_that_would_reach_the_flags_are_refused():
+    """2^29 - 1 table entries and more: a need of that many pages would set the
+    bits that stand beside it. (The tables are never read: one row of them is
+    described over a small buffer, and every call is refused on the host.)"""
+    lib, i32 = _lib.load(), torch.int32
+    lens, refs = torch.zeros(1, dtype=i32), torch.zeros(7, dtype=i32)
+    one, data = torch.zeros(1, dtype=i32), torch.zeros(2, 7, 2, 1, 8)
+
+    def table(w):
+        t = _lib.AdaTensor.from_buffer_copy(T(torch.zeros(1, 1, dtype=i32)))
+        t.shape[1] = w
+        return bytes(t)
+
+    p = _planes(data)
+    for w, rc in ((2 ** 29 - 1, UNSUPPORTED), (2 ** 29, UNSUPPORTED), (2 ** 30, UNSUPPORTED), (2 ** 29 - 2, WORKSPACE)):
+        pool = (table(w), T(lens), T(refs))
+        assert lib.ada_pages_reserve(p, *pool, 1, T(one), T(one), T(one), None, 0, None) == rc
+        assert lib.ada_pages_copy(p, *pool, 1, T(one), T(one), T(one), None, 0, None) == rc
+        assert lib.ada_pages_compact(p, *pool, 1, T(one), None, 0, None) == rc
+    assert lib.ada_pages_free(table(2 ** 29), T(lens), T(refs), 1, T(one), None) == UNSUPPORTED
+
+
 def test_scores_refuse_before_any_device_work():
     lib = _lib.load()
     z, t = torch.zeros(1, 3, 10), torch.zeros(3, dtype=torch.int64)
