@@ -63,7 +63,7 @@ __device__ void tile_prefix(const PagedAttnLaunch& L, int* pref, int* warp_sums)
     const int b0 = min(tid * per, L.B), b1 = min(b0 + per, L.B);
     int sum = 0;
     for (int b = b0; b < b1; ++b) {
-        const int tiles = (seq_length(L, b) + kTile - 1) / kTile;
+        const int tiles = static_cast<int>((static_cast<uint32_t>(seq_length(L, b)) + (kTile - 1)) / kTile);  // (up to 2^31 - 1 keys)
         const int n = tiles > 0 ? tiles + kLead : 0;
         pref[b] = n;
         sum += n;

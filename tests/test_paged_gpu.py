@@ -264,6 +264,26 @@ def test_offsets_past_32_bits(cuda_device):
     del k, v
 
 
+@pytest.mark.parametrize("dtype,page,width", [(torch.float32, 42966, 49981), (torch.bfloat16, 38872, 55245)])
+def test_lengths_up_to_the_last_32_bit_number(dtype, page, width, cuda_device):
+    """2^31 - 2 and 2^31 - 8 keys, all of them the one page's: keys of 0 and values
+    of 1 give 1 and log n. Every sum within a warp counts ones exactly (below
+    2^24 a lane); the 296 x 8 pieces join in as many roundings of 2^-24 at most,
+    lse rounds its logarithm to 2^-23 of itself besides."""
+    dev = cuda_device
+    n = page * width
+    assert 2 ** 31 - 32 < n < 2 ** 31
+    d = 8 if dtype == torch.float32 else 64
+    k = torch.zeros(1, 1, page, d, dtype=dtype, device=dev)
+    out, lse = ada.paged_attention(torch.ones(1, 1, d, dtype=dtype, device=dev), k, torch.ones_like(k),
+                                   torch.zeros(1, width, dtype=torch.int32, device=dev),
+                                   torch.tensor([n], dtype=torch.int32, device=dev), return_lse=True)
+    _lib.poll_device_status(dev)
+    joins = 296 * 8 * 2.0 ** -24
+    assert (out.double() - 1).abs().max().item() <= joins + HALF[dtype]
+    assert abs(lse.item() - math.log(n)) <= joins + 2.0 ** -22 * math.log(n)
+
+
 def test_bad_ids_are_left_out_and_recorded(cuda_device):
     dev = cuda_device
     g = torch.Generator().manual_seed(7)
