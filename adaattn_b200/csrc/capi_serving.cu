@@ -370,7 +370,7 @@ int ada_paged_attn(const AdaTensor* q, const AdaTensor* k_pages, const AdaTensor
         L.mask.dtype = key_mask->dtype;
         L.mask.s[0] = row_stride(key_mask, 0);
         L.mask.s[1] = row_stride(key_mask, 1);
-        L.mask_len = key_mask->shape[1];
+        L.mask_len = std::min(key_mask->shape[1], kMaxInt);  // (no sequence is longer)
     }
     L.k_scale = given(k_scale) ? static_cast<const float*>(k_scale->data) : nullptr;
     L.v_scale = given(v_scale) ? static_cast<const float*>(v_scale->data) : nullptr;

@@ -284,6 +284,20 @@ def test_lengths_up_to_the_last_32_bit_number(dtype, page, width, cuda_device):
     assert abs(lse.item() - math.log(n)) <= joins + 2.0 ** -22 * math.log(n)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_masks_longer_than_any_sequence(dtype, cuda_device):
+    """A mask described over 2^31 + 5 keys (one element, expanded) hides them all."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(14)
+    k, v, table, ln = (t.to(dev) for t in build_pool([40], 16, 2, 64, dtype, g))
+    q = torch.randn(1, 4, 64, generator=g).to(dtype).to(dev)
+    m = torch.zeros(1, 1, dtype=torch.bool, device=dev).expand(1, 2 ** 31 + 5)
+    out, lse = ada.paged_attention(q, k, v, table, ln, key_mask=m, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    open_ = ada.paged_attention(q, k, v, table, ln, key_mask=~m[:, :1].expand(1, 2 ** 31 + 5))
+    assert torch.equal(open_, ada.paged_attention(q, k, v, table, ln))
+
+
 def test_bad_ids_are_left_out_and_recorded(cuda_device):
     dev = cuda_device
     g = torch.Generator().manual_seed(7)
