@@ -305,6 +305,8 @@ struct BwdLaunch {
 int launch_attn_bwd(const BwdLaunch& L, cudaStream_t stream);
 
 // --- paged key-value cache --------------------------------------------------------
+constexpr int kPagedTile = 32;  // keys per tile of paged attention
+constexpr int kPagedLead = 6;   // places before a unit's tiles (3: the ragged 8-bit batch took 205 us, 6: 197)
 struct PagedAttnLaunch {
     CUtensorMap tk, tv;  // tensor-core path: pages [P, Hkv, page, D], chunk x (up to 128 bytes) boxes
     int tc;              // 1: the tensor-core kernel serves the call
@@ -335,7 +337,7 @@ struct PagedAttnLaunch {
     int64_t os[2];
     float* lse;          // [B, H] or null
     int64_t n_cta;
-    int* pref;           // workspace: [B + 1] tiles before each sequence
+    int* pref;           // workspace: [B + 1] places (leads and tiles) before each sequence
     float* part_ml;      // workspace: [n_cta][2][GB][2]
     float* part_acc;     // workspace: [n_cta][2][GB][D]
     unsigned int* status;

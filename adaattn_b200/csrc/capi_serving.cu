@@ -324,6 +324,9 @@ int ada_paged_attn(const AdaTensor* q, const AdaTensor* k_pages, const AdaTensor
     if ((rc = check_width(page_table, page))) return rc;
     if (H < 1 || H % Hkv) return fail(ADA_ERR_SHAPE, "%lld query heads do not divide over %lld key/value heads", (long long)H, (long long)Hkv);
     if (B > kMaxBatch) return fail(ADA_ERR_UNSUPPORTED, "at most %lld sequences per call", (long long)kMaxBatch);
+    // the places of all sequences are counted in 32 bits
+    if (B * ((page_table->shape[1] * page + kPagedTile - 1) / kPagedTile + kPagedLead) > kMaxInt)
+        return fail(ADA_ERR_UNSUPPORTED, "the tables of %lld sequences cover 2^36 keys or more", (long long)B);
     const bool picked = given(seqs);
     if (picked && (rc = check_ints(seqs, "seqs", B))) return rc;
     if (!picked && page_table->shape[0] != B) return fail(ADA_ERR_SHAPE, "page_table must have one row per sequence of q");

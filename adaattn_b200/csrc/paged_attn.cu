@@ -27,8 +27,7 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTile = 32;       // keys per tile
-constexpr int kLead = 6;        // places before a unit's tiles (3: the ragged 8-bit batch took 205 us, 6: 197)
+constexpr int kTile = kPagedTile, kLead = kPagedLead;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

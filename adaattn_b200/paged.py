@@ -114,7 +114,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     per head; a visible infinite value may come out as NaN there. A sequence
     without a visible key gives zeros. With ``return_lse`` also the fp32
     [B, H] log-sum-exp of the scores (-inf there). No autograd. Up to 4096
-    sequences per call, head dims up to 128.
+    sequences per call (whose tables cover less than 2^36 keys), head dims up
+    to 128.
     """
     dev = _device_of(q, k_pages, v_pages, page_table, seq_lens, seqs, key_mask, k_scale, v_scale, out)
     _no_grad("paged_attention", q, k_pages, v_pages, key_mask)

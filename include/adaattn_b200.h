@@ -299,7 +299,8 @@ int         ada_record_statistics(const float* summary, AdaTensor* call_count,
 /* out[b, h] = softmax(scale * q[b, h] . K) V over the seq_lens keys of table
  * row seqs[b] (row b when seqs is NULL or its data is): q, out [B, H, D] in
  * one type, which is the pages' unless they are E4M3; H a multiple of Hkv
- * (query heads h of a group of H / Hkv share a key/value head); B <= 4096.
+ * (query heads h of a group of H / Hkv share a key/value head); B <= 4096,
+ * and the B tables together cover less than 2^36 keys (6 more tiles of 32 each).
  * key_mask [B, L] (or [1, L]) bool (nonzero keeps) or floating point (added;
  * -inf hides), for keys j < L, later keys are open. Hidden keys are not read.
  * k_scale, v_scale float32 [Hkv]: an E4M3 page holds value / scale (NULL: 1).

@@ -130,6 +130,27 @@ def test_page_operations_refuse_before_any_device_work():
         _planes(data.transpose(3, 4))
 
 
+def test_batches_whose_places_pass_32_bits_are_refused():
+    """Tiles of 32 keys and 6 places for each sequence, summed over the batch in
+    32 bits. (The tables are described over a small buffer and never read:
+    every call is refused on the host.)"""
+
+    def table(s, w):
+        t = _lib.AdaTensor.from_buffer_copy(T(torch.zeros(1, 1, dtype=torch.int32)))
+        t.shape[0], t.shape[1], t.stride[0] = s, w, w
+        return bytes(t)
+
+    def call(b, w, page=16):
+        q, k = torch.zeros(1, 1, 64).expand(b, 1, 64), torch.zeros(1, 1, page, 64)
+        return _lib.load().ada_paged_attn(T(q), T(k), T(k), table(b, w), T(torch.zeros(b, dtype=torch.int32)), None, None,
+                                          None, None, 1.0, T(torch.zeros(b, 1, 64)), None, None, 0, None)
+
+    at = (2 ** 31 - 1) // 4096 - 6  # tiles per sequence that still fit
+    assert call(4096, 2 * at) == WORKSPACE and call(4096, 2 * at + 1) == UNSUPPORTED
+    assert call(4096, 2 ** 27 - 1) == UNSUPPORTED and call(33, 2 ** 27 - 1) == UNSUPPORTED
+    assert call(1, 2 ** 27 - 1) == WORKSPACE and call(31, 2 ** 27 - 1) == WORKSPACE
+
+
 def test_needs_that_would_reach_the_flags_are_refused():
     """2^29 - 1 table entries and more: a need of that many pages would set the
     bits that stand beside it. (The tables are never read: one row of them is
