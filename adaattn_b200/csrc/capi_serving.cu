@@ -29,7 +29,13 @@ constexpr int64_t kMaxInt = 0x7FFFFFFF;
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 bool is_float(int dtype) { return dtype == ADA_F32 || dtype == ADA_F16 || dtype == ADA_BF16; }
 int elt_bytes(int dtype) { return dtype == ADA_F32 ? 4 : dtype == ADA_E4M3 ? 1 : 2; }
-bool given(const AdaTensor* t) { return t != nullptr && t->data != nullptr; }
+// An optional tensor is omitted when it is null or describes elements at null; one without elements is given.
+bool given(const AdaTensor* t) {
+    if (t == nullptr || t->data != nullptr) return t != nullptr;
+    for (int i = 0; i < t->ndim && i < 4; ++i)
+        if (t->shape[i] == 0) return true;
+    return false;
+}
 
 // SMs of the current device (asked for once per device).
 int sm_count(int* n) {
@@ -329,7 +335,8 @@ int ada_paged_attn(const AdaTensor* q, const AdaTensor* k_pages, const AdaTensor
         return fail(ADA_ERR_UNSUPPORTED, "the tables of %lld sequences cover 2^36 keys or more", (long long)B);
     const bool picked = given(seqs);
     if (picked && (rc = check_ints(seqs, "seqs", B))) return rc;
-    if (!picked && page_table->shape[0] != B) return fail(ADA_ERR_SHAPE, "page_table must have one row per sequence of q");
+    if (!picked && page_table->shape[0] != B)
+        return fail(ADA_ERR_SHAPE, "page_table must have one row per sequence of q");
     if ((rc = check_scales(k_scale, "k_scale", Hkv, k_pages->dtype)) || (rc = check_scales(v_scale, "v_scale", Hkv, k_pages->dtype)))
         return rc;
     if (given(key_mask)) {
@@ -428,7 +435,8 @@ int append(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages, AdaTensor
     if ((rc = check_width(page_table, page))) return rc;
     const bool picked = given(seqs);
     if (picked && (rc = check_ints(seqs, "seqs", B))) return rc;
-    if (!picked && page_table->shape[0] != B) return fail(ADA_ERR_SHAPE, "page_table must have one row per sequence of k");
+    if (!picked && page_table->shape[0] != B)
+        return fail(ADA_ERR_SHAPE, "page_table must have one row per sequence of k");
     if (given(new_tokens) && (rc = check_ints(new_tokens, "new_tokens", B))) return rc;
     if ((rc = check_scales(k_scale, "k_scale", Hkv, k_pages->dtype)) || (rc = check_scales(v_scale, "v_scale", Hkv, k_pages->dtype)))
         return rc;

@@ -297,7 +297,7 @@ int         ada_record_statistics(const float* summary, AdaTensor* call_count,
  * 1..65536 tokens. */
 
 /* out[b, h] = softmax(scale * q[b, h] . K) V over the seq_lens keys of table
- * row seqs[b] (row b when seqs is NULL or its data is): q, out [B, H, D] in
+ * row seqs[b] (row b when seqs is NULL or its data is, unless it is empty): q, out [B, H, D] in
  * one type, which is the pages' unless they are E4M3; H a multiple of Hkv
  * (query heads h of a group of H / Hkv share a key/value head); B <= 4096,
  * and the B tables together cover less than 2^36 keys (6 more tiles of 32 each).

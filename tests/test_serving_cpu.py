@@ -130,6 +130,34 @@ def test_page_operations_refuse_before_any_device_work():
         _planes(data.transpose(3, 4))
 
 
+def test_an_empty_batch_of_picked_sequences_is_none():
+    """A serving loop with nothing to do: no rows of q or k and an empty list of
+    sequences, whatever the table's size. Without a list the table has to be empty as well."""
+    z, none = torch.zeros, torch.zeros(0, dtype=torch.int32)
+    table, mask = z(3, 2, dtype=torch.int32), z(0, 40, dtype=torch.bool)
+    assert _attn(q=z(0, 4, 64), table=table, seqs=none) == 0
+    assert _attn(q=z(0, 4, 64), table=table, seqs=none, mask=mask) == 0
+    assert _attn(q=z(0, 4, 64), table=table) == SHAPE and _attn(q=z(2, 4, 64), table=table, seqs=none) == SHAPE
+    assert _append(k=z(0, 2, 3, 64), table=table, seqs=none) == 0
+    assert _append(k=z(0, 2, 3, 64), table=table, seqs=none, new=none) == 0
+    assert _append(k=z(0, 2, 3, 64), table=table) == SHAPE
+
+
+def test_empty_options_are_no_omitted_ones():
+    """A list, mask or scale without elements is refused where elements are due, not taken for None."""
+    z, none = torch.zeros, torch.zeros(0, dtype=torch.int32)
+    assert _attn(seqs=none) == SHAPE and _append(seqs=none) == SHAPE and _append(new=none) == SHAPE
+    assert _attn(mask=z(0, 40, dtype=torch.bool)) == SHAPE
+    assert _attn(mask=z(2, 0, dtype=torch.bool)) == WORKSPACE  # covers no key: like none
+    k8 = z(5, 2, 16, 64).to(torch.float8_e4m3fn)
+    assert _attn(k=k8, ks=z(0)) == SHAPE and _append(pages=k8, ks=z(0)) == SHAPE
+    absent = bytes(_lib.AdaTensor())
+    lib, t, p = _lib.load(), torch.zeros(2, 4, 64), torch.zeros(5, 2, 16, 64)
+    table, lens = z(2, 3, dtype=torch.int32), z(2, dtype=torch.int32)
+    assert lib.ada_paged_attn(T(t), T(p), T(p), T(table), T(lens), absent, absent, absent, absent, 1.0, T(t.clone()), None,
+                              None, 0, None) == WORKSPACE
+
+
 def test_batches_whose_places_pass_32_bits_are_refused():
     """Tiles of 32 keys and 6 places for each sequence, summed over the batch in
     32 bits. (The tables are described over a small buffer and never read:
