@@ -85,6 +85,17 @@ def _ids(x: Ids, dev: torch.device) -> torch.Tensor:
     return torch.tensor(list(x), dtype=torch.int32, device=dev)
 
 
+_MASK_DTYPES = (torch.bool, torch.uint8, torch.float32, torch.float16, torch.bfloat16)
+
+
+def _mask32(m: torch.Tensor) -> torch.Tensor:
+    """A mask of another floating type in 32 bits; only infinities become infinite (the type's lowest value hides nothing)."""
+    if not m.is_floating_point():
+        raise TypeError(f"key_mask must be bool (True keeps) or floating point (added), got {m.dtype}")
+    top = torch.finfo(torch.float32).max
+    return torch.where(m.isinf(), m, m.clamp(-top, top)).float() if m.dtype == torch.float64 else m.float()
+
+
 def _unit_last(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
@@ -104,7 +115,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     pages have q's dtype (fp32, fp16 or bf16) or are float8_e4m3fn holding
     value / scale with ``k_scale`` / ``v_scale`` float32 [Hkv] (1 when
     omitted). ``key_mask`` [B, L] or [1, L] covers the first L keys, bool
-    (True keeps) or floating point (added; -inf hides); later keys are open
+    (True keeps; uint8 counts as bool) or floating point (added; -inf hides;
+    float64 beyond float32's range counts as its ends); later keys are open
     and hidden keys are not read. ``scale`` defaults to D ** -0.5.
 
     Scores, softmax and sums are fp32, the result is rounded once. On the
@@ -128,9 +140,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if out is None:
         out = torch.empty(b, h, d, dtype=q.dtype, device=dev)
     lse = torch.empty(b, h, dtype=torch.float32, device=dev) if return_lse else None
-    if key_mask is not None and key_mask.dtype not in (torch.bool, torch.uint8, torch.float32, torch.float16,
-                                                       torch.bfloat16):
-        key_mask = key_mask.float()
+    if key_mask is not None and key_mask.dtype not in _MASK_DTYPES:
+        key_mask = _mask32(key_mask)
     lib = _lib.load()
     ws = torch.empty(_attn_workspace(b, h, max(1, k_pages.shape[1]), d), dtype=torch.uint8, device=dev)
     _call("ada_paged_attn", dev, lib.ada_paged_attn, _lib.packed(_unit_last(q)), _lib.packed(k_pages),

@@ -528,3 +528,27 @@ def test_forward_mode_is_refused(cuda_device):
         att = ada.AdaAttention(embed_dim=64, num_heads=2, causal=True, enable_adaptive_rank=False).to(dev).eval()
         with pytest.raises(RuntimeError, match="forward-mode"):
             att.forward_cached(dual(torch.randn(1, 1, 64, device=dev)), c, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_other_mask_types(dtype, cuda_device):
+    """0/1 masks of whole numbers are refused (added, they would hide nothing),
+    uint8 is bool, and a float64 mask of its lowest value everywhere leaves a uniform row as in 32 bits."""
+    dev = cuda_device
+    g = torch.Generator().manual_seed(15)
+    k, v, table, ln = build_pool([50], 16, 2, 64, dtype, g)
+    q = torch.randn(1, 4, 64, generator=g).to(dtype)
+    m = torch.rand(1, 50, generator=g) < 0.5
+    up = [t.to(dev) for t in (q, k, v, table, ln)]
+    run = lambda mask, **kw: ada.paged_attention(*up, key_mask=mask.to(dev), **kw)
+    for whole in (torch.int64, torch.int32, torch.int16, torch.int8):
+        with pytest.raises(TypeError):
+            run(m.to(whole))
+    assert torch.equal(run(m.to(torch.uint8)), run(m))
+    want, want_lse = run(torch.full((1, 50), torch.finfo(torch.float32).min), return_lse=True)
+    got, lse = run(torch.full((1, 50), torch.finfo(torch.float64).min, dtype=torch.float64), return_lse=True)
+    assert torch.equal(got, want) and torch.equal(lse, want_lse) and (got != 0).any()
+    f = torch.randn(1, 50, generator=g).masked_fill(~m, -math.inf)
+    assert torch.equal(run(f.double()), run(f))
+    assert (run(torch.full((1, 50), -math.inf, dtype=torch.float64)) == 0).all()
+    assert torch.isnan(run(torch.full((1, 50), math.nan, dtype=torch.float64)).float()).all()
