@@ -79,7 +79,15 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor, stats: t
     and ``entropy`` as the forward computed them, upstream gradients [A * R]
     or None. Rows of a vocabulary that is no multiple of 16 bytes keep the
     logits' padding in memory."""
+    if logits.dim() != 3:
+        raise ShapeError(f"logits must be 3-D [A, R, V], got {logits.dim()}-D")
+    rows = logits.shape[0] * logits.shape[1]
     ups = [None if g is None else g.float().contiguous() for g in (grad_logprobs, grad_entropy, grad_lse)]
+    for name, t, shape in (("stats", stats, (rows, 2)), ("entropy", entropy, (rows,)), ("grad_logprobs", ups[0], (rows,)),
+                           ("grad_entropy", ups[1], (rows,)), ("grad_lse", ups[2], (rows,))):
+        if t is not None and (t.shape != shape or t.dtype != torch.float32):
+            raise ShapeError(f"{name} must be float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    stats, entropy = stats.contiguous(), entropy.contiguous()
     dev = _device_of(logits, tokens, stats, entropy, *ups)
     _no_tangent("token_logprobs_backward", logits, stats, entropy, *ups)
     grad = _grad_like(logits)

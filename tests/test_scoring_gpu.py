@@ -484,3 +484,19 @@ def test_forward_mode_is_refused(cuda_device):
         assert torch.equal(ada.token_logprobs(z, t).logprobs, want.logprobs)  # no tangent here
     with pytest.raises(Exception):
         torch.func.jvp(lambda x: ada.token_logprobs(x, t).lse, (z,), (z,))
+
+
+def test_gradient_takes_strided_statistics(cuda_device):
+    """Statistics and entropies read through strides give the gradient of their values."""
+    dev = cuda_device
+    z, t = _make(6, 700, torch.float32)
+    zd, td = z.to(dev), t.to(dev)
+    r = ada.token_logprobs(zd, td)
+    m = zd.amax(-1)
+    ups = torch.randn(6, generator=torch.Generator().manual_seed(1)).to(dev)
+    stats = torch.stack([m, r.lse - m], 1)
+    want = token_logprobs_backward(zd[None], td, stats, r.entropy, ups)
+    wide = torch.full((6, 4), math.nan, device=dev)
+    wide[:, ::2] = stats
+    ent = torch.stack([r.entropy, r.entropy * math.nan], 1)
+    assert torch.equal(token_logprobs_backward(zd[None], td, wide[:, ::2], ent[:, 0], ups), want)

@@ -10,6 +10,7 @@ import torch
 import adaattn_b200 as ada
 from adaattn_b200 import _lib
 from adaattn_b200.paged import _planes
+from adaattn_b200.scoring import token_logprobs_backward
 from serving_util import PoolModel, attend64, build_pool
 
 pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
@@ -223,6 +224,23 @@ def test_scores_refuse_before_any_device_work():
     assert lib.ada_token_logprobs_bwd(T(z), T(t), -100, p[0], p[1], None, None, None, T(grad), None) == SHAPE
     assert lib.ada_token_logprobs_bwd(T(z), T(t), -100, p[0], p[1], None, None, None, T(z.half()), None) == DTYPE
     assert lib.ada_token_logprobs_bwd(T(z), T(t), -100, None, p[1], None, None, None, T(z), None) == INVALID
+
+
+def test_gradient_arguments_are_checked():
+    """The kernel reads a statistic pair, an entropy and an upstream gradient per row, whatever their tensors hold."""
+    z, t = torch.zeros(2, 3, 10), torch.zeros(6, dtype=torch.int64)
+    stats, ent, up = torch.zeros(6, 2), torch.zeros(6), torch.zeros(6)
+
+    def call(z=z, stats=stats, ent=ent, **ups):
+        return token_logprobs_backward(z, t, stats, ent, **ups)
+
+    for bad in (dict(z=z[0]), dict(stats=stats[:5]), dict(stats=stats[:, 0]), dict(stats=stats.double()),
+                dict(ent=ent[:1]), dict(ent=ent.half()), dict(ent=ent[:, None]), dict(grad_logprobs=up[:2]),
+                dict(grad_entropy=up.view(2, 3)), dict(grad_lse=torch.zeros(()))):
+        with pytest.raises(ada.ShapeError):
+            call(**bad)
+    with pytest.raises(RuntimeError, match="CUDA"):  # all right but for the device
+        call(grad_logprobs=up.double())
 
 
 def test_host_tensors_are_refused():
