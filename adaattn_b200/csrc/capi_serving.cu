@@ -84,6 +84,24 @@ int check_table(const AdaTensor* table, const AdaTensor* lens) {
     return check_ints(lens, "seq_lens", table->shape[0]);
 }
 
+// A tensor that is written must hold each element once: along the dimensions
+// in the order of their strides, each step goes past all that is inside it.
+int check_apart(const AdaTensor* t, const char* name) {
+    int order[4], n = 0;
+    for (int i = 0; i < t->ndim; ++i) {
+        if (t->shape[i] == 0) return ADA_OK;
+        if (t->shape[i] > 1) order[n++] = i;
+    }
+    auto step = [&](int i) { return t->stride[i] < 0 ? -t->stride[i] : t->stride[i]; };
+    std::sort(order, order + n, [&](int a, int b) { return step(a) < step(b); });
+    int64_t span = 1;
+    for (int i = 0; i < n; ++i) {
+        if (step(order[i]) < span) return fail(ADA_ERR_LAYOUT, "%s overlaps itself", name);
+        span += (t->shape[order[i]] - 1) * step(order[i]);
+    }
+    return ADA_OK;
+}
+
 int64_t row_stride(const AdaTensor* t, int i) { return t->shape[i] > 1 ? t->stride[i] : 0; }
 
 // Every row of a view starts on an `align`-byte boundary.
@@ -344,7 +362,9 @@ int ada_paged_attn(const AdaTensor* q, const AdaTensor* k_pages, const AdaTensor
             return fail(ADA_ERR_SHAPE, "key_mask must be [B, L]");
         if (key_mask->dtype != ADA_BOOL && !is_float(key_mask->dtype)) return fail(ADA_ERR_DTYPE, "key_mask must be bool or floating point");
     }
+    if ((rc = check_apart(out, "out"))) return rc;
     if (B == 0) return ADA_OK;
+    if (out->data == q->data) return fail(ADA_ERR_LAYOUT, "out shares q's memory");
     if (workspace == nullptr || workspace_bytes < ada_paged_attn_workspace_bytes(B, H, Hkv, D))
         return fail(ADA_ERR_WORKSPACE, "paged attention workspace too small");
     unsigned int* st;
@@ -440,6 +460,7 @@ int append(const AdaTensor* k, const AdaTensor* v, AdaTensor* k_pages, AdaTensor
     if (given(new_tokens) && (rc = check_ints(new_tokens, "new_tokens", B))) return rc;
     if ((rc = check_scales(k_scale, "k_scale", Hkv, k_pages->dtype)) || (rc = check_scales(v_scale, "v_scale", Hkv, k_pages->dtype)))
         return rc;
+    if ((rc = check_apart(k_pages, "k_pages")) || (rc = check_apart(v_pages, "v_pages"))) return rc;
     if (B == 0 || N == 0) return ADA_OK;
     if (N > kMaxInt || B > kMaxInt) return fail(ADA_ERR_UNSUPPORTED, "too many tokens");
     unsigned int* st;
@@ -628,6 +649,7 @@ int ada_token_logprobs_bwd(const AdaTensor* logits, const AdaTensor* tokens, int
     if (grad->dtype != logits->dtype) return fail(ADA_ERR_DTYPE, "grad must have the logits' dtype");
     for (int i = 0; i < 3; ++i)
         if (grad->shape[i] != logits->shape[i]) return fail(ADA_ERR_SHAPE, "grad and logits differ in extent %d", i);
+    if ((rc = check_apart(grad, "grad"))) return rc;
     if (L.rows == 0) return ADA_OK;
     if (stats == nullptr || entropy == nullptr) return fail(ADA_ERR_INVALID, "null argument");
     L.ignore = ignore_index;

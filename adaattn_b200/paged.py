@@ -125,7 +125,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     over the others, and q over 8-bit pages to fp16's bits after a power of two
     per head; a visible infinite value may come out as NaN there. A sequence
     without a visible key gives zeros. With ``return_lse`` also the fp32
-    [B, H] log-sum-exp of the scores (-inf there). No autograd. Up to 4096
+    [B, H] log-sum-exp of the scores (-inf there). ``out`` shares no memory with
+    the inputs or with itself. No autograd. Up to 4096
     sequences per call (whose tables cover less than 2^36 keys), head dims up
     to 128.
     """

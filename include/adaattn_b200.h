@@ -305,7 +305,7 @@ int         ada_record_statistics(const float* summary, AdaTensor* call_count,
  * -inf hides), for keys j < L, later keys are open. Hidden keys are not read.
  * k_scale, v_scale float32 [Hkv]: an E4M3 page holds value / scale (NULL: 1).
  * lse float32 [B, H] or NULL: log sum exp of the scores (-inf and a zero
- * output row where no key is visible). */
+ * output row where no key is visible). out shares no memory with q or the pages. */
 size_t      ada_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim);
 int         ada_paged_attn(const AdaTensor* q, const AdaTensor* k_pages, const AdaTensor* v_pages,
                            const AdaTensor* page_table, const AdaTensor* seq_lens, const AdaTensor* seqs,

@@ -226,6 +226,25 @@ def test_scores_refuse_before_any_device_work():
     assert lib.ada_token_logprobs_bwd(T(z), T(t), -100, None, p[1], None, None, None, T(z), None) == INVALID
 
 
+def test_what_is_written_may_not_overlap_itself():
+    """Expanded or interlaced outputs, pages and gradients (several elements in one place) and an output in q's
+    memory are refused; transposed, sliced and padded ones are not."""
+    z = torch.zeros
+    q = z(2, 4, 64)
+    assert _attn(out=z(1, 4, 64).expand(2, 4, 64)) == LAYOUT and _attn(out=z(2, 1, 64).expand(2, 4, 64)) == LAYOUT
+    assert _attn(out=z(1000).as_strided((2, 4, 64), (128, 64, 1))) == LAYOUT
+    assert _attn(out=z(1000).as_strided((2, 4, 64), (256, 63, 1))) == LAYOUT
+    assert _attn(q=q, out=q) == LAYOUT
+    for out in (z(4, 2, 64).transpose(0, 1), z(2, 8, 64)[:, ::2], z(2, 4, 80)[..., :64], z(2, 4, 2, 64)[:, :, 1]):
+        assert _attn(out=out) == WORKSPACE
+    for pages in (z(1, 2, 16, 64).expand(5, 2, 16, 64), z(5, 1, 16, 64).expand(5, 2, 16, 64), z(5, 2, 1, 64).expand(5, 2, 16, 64)):
+        assert _append(pages=pages) == LAYOUT
+    assert _append(k=z(2, 2, 0, 64), pages=z(5, 16, 2, 64).transpose(1, 2)) == 0
+    lib, t, zl, o = _lib.load(), z(3, dtype=torch.int64), z(1, 3, 10), z(3, 2)
+    assert lib.ada_token_logprobs_bwd(T(zl), T(t), -100, o.data_ptr(), o.data_ptr(), None, None, None,
+                                      T(z(1, 1, 10).expand(1, 3, 10)), None) == LAYOUT
+
+
 def test_gradient_arguments_are_checked():
     """The kernel reads a statistic pair, an entropy and an upstream gradient per row, whatever their tensors hold."""
     z, t = torch.zeros(2, 3, 10), torch.zeros(6, dtype=torch.int64)
