@@ -38,7 +38,7 @@ def _rows3(t: torch.Tensor) -> torch.Tensor:
         return t[None]
     if t.dim() == 3:
         return t
-    return t.reshape(t.shape[0], -1, t.shape[-1])
+    return t.reshape(t.shape[0], t.shape[1:-1].numel(), t.shape[-1])
 
 
 def _grad_like(z3: torch.Tensor) -> torch.Tensor:

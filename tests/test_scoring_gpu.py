@@ -500,3 +500,13 @@ def test_gradient_takes_strided_statistics(cuda_device):
     wide[:, ::2] = stats
     ent = torch.stack([r.entropy, r.entropy * math.nan], 1)
     assert torch.equal(token_logprobs_backward(zd[None], td, wide[:, ::2], ent[:, 0], ups), want)
+
+
+@pytest.mark.parametrize("lead", [(0, 2, 3), (2, 0, 3), (0, 5), (0,)])
+def test_no_rows_of_any_leading_dimensions(lead, cuda_device):
+    dev = cuda_device
+    z = torch.zeros(*lead, 9, device=dev, requires_grad=True)
+    r = ada.token_logprobs(z, torch.zeros(lead, dtype=torch.int64, device=dev), top_k=2)
+    assert r.logprobs.shape == lead and r.top_tokens.shape == (*lead, 2)
+    grad, = torch.autograd.grad((r.logprobs.sum(), r.entropy.sum()), z)
+    assert grad.shape == z.shape

@@ -10,7 +10,7 @@ import torch
 import adaattn_b200 as ada
 from adaattn_b200 import _lib
 from adaattn_b200.paged import _planes
-from adaattn_b200.scoring import token_logprobs_backward
+from adaattn_b200.scoring import _rows3, token_logprobs_backward
 from serving_util import PoolModel, attend64, build_pool
 
 pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
@@ -243,6 +243,16 @@ def test_what_is_written_may_not_overlap_itself():
     lib, t, zl, o = _lib.load(), z(3, dtype=torch.int64), z(1, 3, 10), z(3, 2)
     assert lib.ada_token_logprobs_bwd(T(zl), T(t), -100, o.data_ptr(), o.data_ptr(), None, None, None,
                                       T(z(1, 1, 10).expand(1, 3, 10)), None) == LAYOUT
+
+
+@pytest.mark.parametrize("lead", [(0, 2, 3), (2, 0, 3), (2, 3, 0), (0, 0, 0), (2, 3, 4), (2, 0), (0,), ()])
+def test_rows_of_any_leading_dimensions(lead):
+    """Logits without rows have three dimensions like all others."""
+    z = torch.zeros(*lead, 9)
+    rows = _rows3(z)
+    assert rows.dim() == 3 and rows.shape[0] * rows.shape[1] == z.numel() // 9 and rows.shape[2] == 9
+    if len(lead) > 1:
+        assert rows.shape[0] == lead[0]
 
 
 def test_gradient_arguments_are_checked():
