@@ -413,7 +413,7 @@ struct LogprobLaunch {
     float* logprobs;     // [rows]
     float* entropy;      // [rows]
     float* lse;          // [rows]
-    float* stats;        // [rows][2]: row maximum, log of the sum of exp(z - maximum)
+    float* stats;        // [rows][2]: row maximum, log of the sum of exp(z - maximum); forward: or null
     float* top_logprobs; // [rows][top]
     int64_t* top_tokens;
     int cluster;         // CTAs per row

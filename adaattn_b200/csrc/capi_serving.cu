@@ -617,7 +617,7 @@ int ada_token_logprobs(const AdaTensor* logits, const AdaTensor* tokens, int64_t
     if (top_k < 0 || top_k > 64) return fail(ADA_ERR_UNSUPPORTED, "top_k %d outside [0, 64]", top_k);
     if (top_k > L.V) return fail(ADA_ERR_SHAPE, "top_k %d exceeds the vocabulary", top_k);
     if (L.rows == 0) return ADA_OK;
-    if (logprobs == nullptr || entropy == nullptr || lse == nullptr || stats == nullptr ||
+    if (logprobs == nullptr || entropy == nullptr || lse == nullptr ||
         (top_k > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
         return fail(ADA_ERR_INVALID, "null output");
     L.ignore = ignore_index;

@@ -642,8 +642,10 @@ __global__ void __launch_bounds__(kT, DT == ADA_F32 ? 0 : TOP ? 6 : 8) token_log
         L.logprobs[row] = lp;
         L.entropy[row] = ls - mean;
         L.lse[row] = a.m + ls;
-        L.stats[2 * row] = a.m;
-        L.stats[2 * row + 1] = ls;
+        if (L.stats != nullptr) {
+            L.stats[2 * row] = a.m;
+            L.stats[2 * row + 1] = ls;
+        }
     }
     if constexpr (TOP) {
         for (int i = threadIdx.x; i < k; i += kT) {

@@ -53,19 +53,18 @@ def _grad_like(z3: torch.Tensor) -> torch.Tensor:
     return torch.empty(a, r, ld, dtype=z3.dtype, device=z3.device)[..., :v]
 
 
-def _forward(z3: torch.Tensor, tokens: torch.Tensor, top_k: int, ignore_index: int, views: bool = True):
-    """``views``: the three vectors and the statistics may share one buffer."""
+def _forward(z3: torch.Tensor, tokens: torch.Tensor, top_k: int, ignore_index: int, with_stats: bool = False):
+    """Each output in memory of its own: views of one buffer would share a
+    version counter, and autograd refuse to change one in place beside another."""
     dev = z3.device
     rows = z3.shape[0] * z3.shape[1]
-    if views:
-        lp, ent, lse, stats, _ = torch.empty(5, rows, dtype=torch.float32, device=dev).unbind(0)
-    else:
-        lp, ent, lse = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(3))
-        stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
+    lp = torch.empty(rows, dtype=torch.float32, device=dev)
+    ent, lse = lp.new_empty(rows), lp.new_empty(rows)
+    stats = lp.new_empty(rows, 2) if with_stats else None
     top_lp = torch.empty(rows, top_k, dtype=torch.float32, device=dev) if top_k else None
     top_id = torch.empty(rows, top_k, dtype=torch.int64, device=dev) if top_k else None
     _call("ada_token_logprobs", dev, _lib.load().ada_token_logprobs, _lib.packed(z3), _lib.packed(tokens),
-          int(ignore_index), int(top_k), lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), stats.data_ptr(),
+          int(ignore_index), int(top_k), lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), _lib.ptr(stats),
           _lib.ptr(top_lp), _lib.ptr(top_id))
     return lp, ent, lse, top_lp, top_id, stats
 
@@ -101,7 +100,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, ignore_index):
         z3 = _rows3(logits)
-        lp, ent, lse, top_lp, top_id, stats = _forward(z3, tokens, top_k, ignore_index, views=False)
+        lp, ent, lse, top_lp, top_id, stats = _forward(z3, tokens, top_k, ignore_index, with_stats=True)
         ctx.save_for_backward(logits, tokens, stats, ent)
         ctx.ignore_index = ignore_index
         ctx.set_materialize_grads(False)

@@ -375,7 +375,7 @@ int         ada_pages_compact(AdaTensor* pages, AdaTensor* page_table, AdaTensor
  *   entropy, lse  of softmax(row): -sum p log p; log sum exp
  *   top_logprobs, top_tokens [rows, top_k] (NULL when top_k = 0; top_k <= 64):
  *                 the largest in order, equal logits by lowest token, NaN first
- *   stats         [rows, 2] row maximum and log sum exp(z - maximum), for the gradient
+ *   stats         [rows, 2] row maximum and log sum exp(z - maximum), for the gradient (NULL: not wanted)
  * all float32 (top_tokens int64). A logit of -inf has probability 0; a row of
  * -inf alone, or one with +inf or NaN, gives NaN (lse: -inf for the former). */
 int         ada_token_logprobs(const AdaTensor* logits, const AdaTensor* tokens, int64_t ignore_index,

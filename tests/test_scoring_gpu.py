@@ -510,3 +510,24 @@ def test_no_rows_of_any_leading_dimensions(lead, cuda_device):
     assert r.logprobs.shape == lead and r.top_tokens.shape == (*lead, 2)
     grad, = torch.autograd.grad((r.logprobs.sum(), r.entropy.sum()), z)
     assert grad.shape == z.shape
+
+
+def test_outputs_are_tensors_of_their_own(cuda_device):
+    """One may change in place while another waits for a backward pass, or take part in autograd itself."""
+    dev = cuda_device
+    z, t = _make(4, 300, torch.float32)
+    z, t = z.to(dev), t.to(dev)
+    want = ada.token_logprobs(z, t, top_k=2)
+    w = torch.ones(4, device=dev, requires_grad=True)
+    r = ada.token_logprobs(z, t, top_k=2)
+    loss = (w * r.entropy).sum()
+    r.logprobs.neg_()
+    r.lse.zero_()
+    g, = torch.autograd.grad(loss, w)
+    assert torch.equal(g, want.entropy)
+    r.lse.add_(w)
+    assert r.lse.requires_grad and torch.equal(r.entropy, want.entropy) and torch.equal(r.logprobs, -want.logprobs)
+    assert len({x.untyped_storage().data_ptr() for x in r}) == 5
+    x = z.clone().requires_grad_()  # with autograd the same bits
+    for a, b in zip(ada.token_logprobs(x, t, top_k=2), want):
+        assert torch.equal(a, b)
