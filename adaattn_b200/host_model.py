@@ -175,7 +175,10 @@ class AdaptiveTransformer(nn.Module):
     def score(self, input_ids: torch.Tensor, *, top_k: int = 0, attention_mask=None) -> TokenLogprobs:
         """Log probability of each token of input_ids [B, N] after the first
         given those before it ([B, N - 1]), with entropies and top_k
-        alternatives (``token_logprobs``); differentiable. For a causal decoder."""
+        alternatives (``token_logprobs``); differentiable. The decoder must be
+        causal, or attention_mask keep each token from itself and what follows."""
+        if attention_mask is None and not all(b.attention.causal for b in self.blocks):
+            raise RuntimeError("score needs a causal decoder (causal=True) or a mask: each token would see itself")
         logits = self.forward(input_ids, attention_mask=attention_mask)
         return token_logprobs(logits[:, :-1], input_ids[:, 1:], top_k=top_k)
 

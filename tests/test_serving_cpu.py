@@ -9,6 +9,7 @@ import torch
 
 import adaattn_b200 as ada
 from adaattn_b200 import _lib
+from adaattn_b200.host_model import AdaptiveTransformer
 from adaattn_b200.paged import _planes
 from adaattn_b200.scoring import _rows3, token_logprobs_backward
 from serving_util import PoolModel, attend64, build_pool
@@ -317,3 +318,15 @@ def test_the_references_themselves():
     assert m.compact() == 3 and m.table.tolist() == [[2, 0], [2, 1], [-1, -1]]
     m.free([0, 1])
     assert m.refs.sum() == 0
+
+
+def test_scores_of_a_decoder_that_sees_ahead_are_refused():
+    """A decoder built without causal=True gives a token's position the token itself; a mask may close it."""
+    m = AdaptiveTransformer(50, 32, 2, 2, 64, max_seq_len=16, dropout=0.0)
+    ids = torch.zeros(1, 4, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="causal"):
+        m.score(ids)
+    m.forward = lambda ids, attention_mask=None: torch.zeros(*ids.shape, 50)  # (the attention has no CPU path)
+    for kw in (dict(attention_mask=torch.ones(4, 4).tril()[None, None]),):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            m.score(ids, **kw)

@@ -263,3 +263,19 @@ def _fresh(cache):
     c = ada.PagedKVCache(1, p, page, hkv, d, max_sequences=4, max_pages_per_sequence=4, dtype=cache.dtype)
     c.reserve([1], [12])
     return c
+
+
+def test_score_through_a_mask(cuda_device):
+    """A decoder without causal=True scores through a causal mask; without one it is refused."""
+    dev = cuda_device
+    m = _model(dev, torch.float32)
+    ids = torch.randint(0, V, (2, 20), generator=torch.Generator().manual_seed(10)).to(dev)
+    with torch.no_grad():
+        want = m.score(ids)
+        for b in m.blocks:
+            b.attention.causal = False
+        with pytest.raises(RuntimeError, match="causal"):
+            m.score(ids)
+        got = m.score(ids, attention_mask=torch.ones(2, 1, 20, 20, dtype=torch.bool, device=dev).tril())
+    # the same sums of 20 keys; logits of size below 1 to fp32 roundings through three layers
+    assert (got.logprobs - want.logprobs).abs().max().item() <= 2 * _bar(torch.float32) + 2.0 ** -20
