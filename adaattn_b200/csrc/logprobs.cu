@@ -23,7 +23,8 @@
 // TB/s; fp32 473 us, 7.0 TB/s), 385 us with 5 and 437 us with 20 alternatives.
 // The gradient runs at 6.5 TB/s of reads and writes. Logits are clamped from below (-2^100;
 // fp16: its lowest value) so that -inf stays out of the weighted sum; a row
-// whose maximum is beyond 2^15 in size is done again by the plain formulas.
+// whose maximum is beyond 2^15 in size is done again by the plain formulas (16384
+// such rows 742 us instead of 303).
 //
 // Top k (k <= 64): candidates are 64-bit keys, the value's order above the
 // inverted column, so all keys differ and equal values rank by lowest index.

@@ -4,8 +4,9 @@
 //   s_j = scale * ks_g * (q_h . k_j) + add_j      over visible keys j < len_b
 //   o_h = vs_g * sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  m = max_j s_j
 // (ks, vs: the scales of an 8-bit cache; add: a float key mask). A key hidden
-// by a bool mask or by -inf is never read, so what its page holds does not
-// matter; a sequence with no visible key gives zeros and lse = -inf.
+// by a bool mask or by -inf takes no part, whatever its page holds (the
+// CUDA-core kernel does not read it, the other one puts zeros in its values'
+// place); a sequence with no visible key gives zeros and lse = -inf.
 //
 // Each key and value is read once per block of up to 8 query heads and costs 4
 // multiply-adds per head and element: the cache's bytes bound the operator.
@@ -312,9 +313,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 // a time. A lane's partial products for GB heads are summed over its LPK
 // lanes by halving exchanges that leave head (lane mod GB) with each lane:
 // GB - 1 + log2(LPK / GB) shuffles for GB sums instead of GB log2(LPK).
-// About 90 instructions per key of 8 heads, and its loads go through registers:
-// 1 TB/s on 16-bit and 0.5 TB/s on 8-bit pages, so it serves what the
-// tensor-core kernel does not take (fp32, other head dims, unaligned rows).
+// About 90 instructions per key of 8 heads, and its loads go through registers.
+// 16 sequences of 8192 keys, 32/8 heads: fp32 heads of 128 297 us (3.6 TB/s),
+// bf16 heads of 80 and 96 600 us (0.6 TB/s), of 32 172 us (0.8), E4M3 heads of
+// 80 533 us (0.3), bf16 heads of 128 in pages of 5 598 us (0.9). So it serves
+// what the tensor-core kernel does not take (fp32, other head dims, unaligned
+// rows and pages that are no multiple of 8).
 template <int GB, int LPK>
 __device__ __forceinline__ float sum_heads(float (&x)[GB], int lane) {
     int width = LPK;
@@ -549,10 +553,15 @@ int launch_simt_gb(const PagedAttnLaunch& L, cudaStream_t stream) {
 //
 // Every warp runs alone: it requests its own tiles by TMA, STAGES ahead (also
 // across units), into its own ring, and no barrier is shared between warps
-// until the join at the end. One CTA per SM with 192 KB of tiles in flight.
+// until the join at the end. One CTA per SM with the stages that fit beside the
+// join: 192 KB of tiles in flight, 128 KB for 8-bit heads of 128 and for wide
+// groups of heads of 128 (their third stage misses the space by little).
 // Measured: 131071 keys of 8 heads of 128 in fp16 (537 MB) 102 us a call, 5.3 TB/s
 // (82 us at the copy rate); 64 sequences up to 16384 keys in E4M3 (1.07 GB)
-// 190 us, 5.7 TB/s; the CUDA-core kernel above took 541 us and 2.02 ms.
+// 190 us, 5.7 TB/s; the CUDA-core kernel above took 541 us and 2.02 ms. Shorter
+// units cost more each: 1000 sequences of 160 keys, 32/8 heads of 128, 178 us in
+// bf16 (3.7 TB/s) and 121 us in E4M3 (2.7); 128 heads over 8, 16 sequences of 8192
+// keys, 160 us (3.4 TB/s) and 121 us (2.2) where 32 over 8 take 125 and 78.
 template <int KIND, int D, int NT>  // KIND: 0 bf16, 1 fp16, 2 E4M3
 struct TcCfg {
     static constexpr int EB = KIND == 2 ? 1 : 2;
@@ -560,7 +569,7 @@ struct TcCfg {
     static constexpr int NBOX = D * EB / RB;
     static constexpr int HALF = kTile * D * EB;              // K or V bytes of a tile
     static constexpr int TILE = 2 * HALF;
-    static constexpr int WARPS = TILE >= 16384 ? 4 : 8;      // (10 with 2 stages for 8-bit pages: 3 % slower)
+    static constexpr int WARPS = TILE >= 16384 ? 4 : 8;      // (8-bit heads of 128: 10, with the same 2 stages, 3 % slower)
     static constexpr int STAGES = TILE >= 8192 ? 3 : 6;      // at most; fewer when the rest needs the space
     static constexpr int GB = 8 * NT;
     static constexpr int PART = GB * D;                      // floats a warp leaves per slot

@@ -117,7 +117,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     omitted). ``key_mask`` [B, L] or [1, L] covers the first L keys, bool
     (True keeps; uint8 counts as bool) or floating point (added; -inf hides;
     float64 beyond float32's range counts as its ends); later keys are open
-    and hidden keys are not read. ``scale`` defaults to D ** -0.5.
+    and what hidden keys hold does not matter. ``scale`` defaults to D ** -0.5.
 
     Scores, softmax and sums are fp32, the result is rounded once. On the
     tensor cores (16- and 8-bit pages, heads of 64 or 128) a probability is
@@ -216,7 +216,8 @@ def reserve_pages(pages: torch.Tensor, page_table: torch.Tensor, seq_lens: torch
     that share it keeps it when they are all its holders). Returns int32
     [n]: the tokens granted, new_tokens[i], or 0 for a sequence that was left
     as it was because the needs up to and including its own exceed the free
-    pages. Free pages are handed out lowest id first."""
+    pages, or (recorded in the status word) because they exceed its table row
+    or it was named before. Free pages are handed out lowest id first."""
     dev = _device_of(pages, page_table, seq_lens, ref_counts, seqs, new_tokens)
     granted = torch.empty(seqs.shape, dtype=torch.int32, device=dev)
     ws = _workspace(page_table, ref_counts, seqs.numel())

@@ -302,7 +302,7 @@ int         ada_record_statistics(const float* summary, AdaTensor* call_count,
  * (query heads h of a group of H / Hkv share a key/value head); B <= 4096,
  * and the B tables together cover less than 2^36 keys (6 more tiles of 32 each).
  * key_mask [B, L] (or [1, L]) bool (nonzero keeps) or floating point (added;
- * -inf hides), for keys j < L, later keys are open. Hidden keys are not read.
+ * -inf hides), for keys j < L, later keys are open. What hidden keys hold does not matter.
  * k_scale, v_scale float32 [Hkv]: an E4M3 page holds value / scale (NULL: 1).
  * lse float32 [B, H] or NULL: log sum exp of the scores (-inf and a zero
  * output row where no key is visible). out shares no memory with q or the pages. */
